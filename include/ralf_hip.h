@@ -563,6 +563,78 @@ typedef struct RalfPackJob { const void* src; void* dst; int64_t ld; int N, K; i
 int ralf_tlayer_pack(const RalfPackJob* jobs, int njobs, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Serving operators (rope.hip, paged_kv.hip, paged_attention.hip, logits.hip): rotary positions, a key / value cache in pages, attention of new
+ * tokens over it, history-dependent logits in front of ralf_mask_sample.
+ * ------------------------------------------------------------------------------------------- */
+/* rotary positions with several axes: pair j of the first R dims of every head turns by pos[axis[j]][t] * freq[j] radians
+ *   (a, b) -> (a cos - b sin, b cos + a sin);  dims >= R pass through.
+ * x, y [T][H][D] of `dtype` (RALF_F32 / RALF_BF16) with token / head strides in elements (the last dim contiguous); y may be x itself, otherwise the
+ * two must not overlap.  pos int64 [A][pos_as >= T], |pos| < 2^31; freq double [R/2]; axis int32 [R/2] (a pair whose axis is outside [0, A) is not turned).
+ * adjacent: pair j = dims (2j, 2j+1), otherwise (j, R/2 + j).  inverse: the opposite angle (the gradient of the forward). */
+typedef struct RalfRopeDesc {
+    const void* x; void* y; const int64_t* pos; const double* freq; const int* axis;
+    int64_t T, x_ts, x_hs, y_ts, y_hs, pos_as;
+    int H, D, R, A, dtype, adjacent, inverse, pad_;
+} RalfRopeDesc;
+int ralf_rope_axes(const RalfRopeDesc* d, void* stream);
+
+/* key / value cache in pages: k, v [n_pages][heads][page][dim] (contiguous, 16-byte aligned), page in {16, 32, 64, 128, 256}, dim in {32, 64, 128, 256}.
+ * store: RALF_KV_F32 / RALF_KV_BF16 hold the values; RALF_KV_E4M3 / RALF_KV_INT8 hold codes, and k_exp, v_exp uint8 [n_pages][heads][page] the power of two
+ * 2^(byte - 127) that a row's codes are multiples of.  Rule of a row: e = the smallest integer with max|x| <= 448 * 2^e (127 * 2^e for int8), at least
+ * -100; code = x / 2^e rounded to nearest even.  A row that holds an infinity or a NaN is stored as byte 255 and zero codes and reads back as NaN.
+ * table int32 [B][table_ld >= max_pages]: the pages of each sequence; kv_len int32 [B]: its tokens (at most max_pages * page are looked at).
+ * A page id outside [0, n_pages) is never followed: nothing is written there, reads give zeros, attention leaves its keys out. */
+#define RALF_KV_F32 0
+#define RALF_KV_BF16 1
+#define RALF_KV_E4M3 2
+#define RALF_KV_INT8 3
+typedef struct RalfPagedKV {
+    void* k; void* v; void* k_exp; void* v_exp;
+    const int* table; const int* kv_len;
+    int64_t n_pages, table_ld;
+    int page, heads, dim, store, B, max_pages;
+} RalfPagedKV;
+/* k, v [T][heads][dim] of `dtype` (strides in elements, multiples of 8): rows q_start[b] .. q_start[b+1]-1 are the LAST tokens of sequence b (positions
+ * kv_len[b] - n .. kv_len[b] - 1; a negative position is left out).  q_start int32 [B+1], ascending from 0.  Rows at or behind q_start[B] are not stored. */
+int ralf_paged_kv_write(const RalfPagedKV* kv, int dtype, const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
+                        const int* q_start, int64_t T, void* stream);
+/* k, v [rows][heads][dim] contiguous of `dtype`: rows start[b] .. start[b+1]-1 <- positions 0 .. of sequence b (zeros behind kv_len[b]); rows at or behind
+ * start[B] are left as they were.  start int32 [B+1], ascending from 0. */
+int ralf_paged_kv_read(const RalfPagedKV* kv, int dtype, void* k, void* v, const int* start, int64_t rows, void* stream);
+
+/* attention of each sequence's newest tokens over its pages.  q, o [T][q_heads][dim] of `dtype` (RALF_BF16 with pools of bf16 / e4m3 / int8; RALF_F32 with
+ * fp32 / e4m3 / int8), strides in elements, multiples of 8; q_heads a multiple of kv->heads: query head h reads key head h / (q_heads / heads).
+ * Row i of the n = q_start[b+1] - q_start[b] rows of sequence b stands at position P = kv_len[b] - n + i and sees the keys p with
+ *   0 <= p < kv_len[b];  p <= P if causal;  p > P - window if window > 0.
+ * o = sum_p exp(s_p - max s) v_p / sum_p exp(s_p - max s), s = scale * q.k; a row that sees no key (or only scores of -inf) gives zeros.  What a row does
+ * not see does not reach it, infinities and NaN included.  Rows at or behind q_start[B] of o are left as they were.
+ * max_q, max_kv: upper bounds of n and kv_len known to the host (0 = unknown): they steer the split of the work, never the result's definition.
+ * workspace: ralf_paged_attention_workspace_bytes() bytes (0 = none needed), 16-byte aligned, private to this call until it has run. */
+typedef struct RalfPagedAttnDesc {
+    RalfPagedKV kv;
+    const void* q; void* o; const int* q_start;
+    int64_t T, q_ts, q_hs, o_ts, o_hs;
+    int q_heads, dtype, causal, window, max_q, max_kv;
+    float scale; int pad_;
+} RalfPagedAttnDesc;
+size_t ralf_paged_attention_workspace_bytes(const RalfPagedAttnDesc* d);
+int ralf_paged_attention(const RalfPagedAttnDesc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* logits in front of the token choice: for row b with history tokens[b][0 .. len[b]-1] (ids outside [0, V) are skipped), c = occurrences of v in it,
+ * c_out = those at index >= prompt_len[b] (NULL: 0):
+ *   x = x > 0 ? x / repetition[b] : x * repetition[b]  where c > 0;   x -= frequency[b] * c_out + (c_out > 0 ? presence[b] : 0);   x += bias[v];
+ *   x = -inf where bit (v & 31) of mask[mask_row[b]][v >> 5] is 0 (mask_row NULL: row b; a mask_row outside [0, mask_rows): no mask).
+ * logits, out [B][V] of `dtype` with row strides (elements); out may be logits itself.  repetition / presence / frequency float [B], bias float [V] or [B][bias_ld]
+ * (bias_ld 0: one row for all), each may be NULL.  len int32 [B] (clamped to [0, L]). */
+typedef struct RalfLogitsDesc {
+    const void* logits; void* out; const int64_t* tokens; const int* len; const int* prompt_len;
+    const float* repetition; const float* presence; const float* frequency; const float* bias; const int* mask; const int* mask_row;
+    int64_t ld_in, ld_out, tok_ld, bias_ld, mask_ld;
+    int B, V, L, mask_rows, dtype, pad_;
+} RalfLogitsDesc;
+int ralf_logits_process(const RalfLogitsDesc* d, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Optimizer (ralf_amd/csrc/optim.hip): clip_grad_norm_ + AdamW on flat fp32 buffers
  * ------------------------------------------------------------------------------------------- */
 int ralf_sumsq(const float* g, int64_t n, float* out, void* stream);                 /* out[0] += sum g^2 (fp32 atomics: order not fixed) */

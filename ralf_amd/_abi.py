@@ -100,6 +100,26 @@ class RalfGemmDesc(ctypes.Structure):
     )
 
 
+class RalfRopeDesc(ctypes.Structure):
+    _fields_ = ([(n, vp) for n in ("x", "y", "pos", "freq", "axis")] + [(n, i64) for n in ("T", "x_ts", "x_hs", "y_ts", "y_hs", "pos_as")]
+                + [(n, i32) for n in ("H", "D", "R", "A", "dtype", "adjacent", "inverse", "pad_")])
+
+
+class RalfPagedKV(ctypes.Structure):
+    _fields_ = ([(n, vp) for n in ("k", "v", "k_exp", "v_exp", "table", "kv_len")] + [(n, i64) for n in ("n_pages", "table_ld")]
+                + [(n, i32) for n in ("page", "heads", "dim", "store", "B", "max_pages")])
+
+
+class RalfPagedAttnDesc(ctypes.Structure):
+    _fields_ = ([("kv", RalfPagedKV)] + [(n, vp) for n in ("q", "o", "q_start")] + [(n, i64) for n in ("T", "q_ts", "q_hs", "o_ts", "o_hs")]
+                + [(n, i32) for n in ("q_heads", "dtype", "causal", "window", "max_q", "max_kv")] + [("scale", f32), ("pad_", i32)])
+
+
+class RalfLogitsDesc(ctypes.Structure):
+    _fields_ = ([(n, vp) for n in ("logits", "out", "tokens", "len", "prompt_len", "repetition", "presence", "frequency", "bias", "mask", "mask_row")]
+                + [(n, i64) for n in ("ld_in", "ld_out", "tok_ld", "bias_ld", "mask_ld")] + [(n, i32) for n in ("B", "V", "L", "mask_rows", "dtype", "pad_")])
+
+
 class RalfWgradJob(ctypes.Structure):
     _fields_ = [("dy", vp), ("x", vp), ("dw", vp), ("rows", i64), ("ld_dy", i64), ("ld_x", i64), ("ld_dw", i64),
                 ("n_out", i32), ("n_in", i32), ("splitk", i32), ("pad", i32), ("db", vp)]
@@ -185,6 +205,12 @@ SIGNATURES.update({
     "ralf_tlayer_fwd": (i32, [ctypes.POINTER(RalfTLayerDesc), vp]),
     "ralf_tlayer_pack": (i32, [ctypes.POINTER(RalfPackJob), i32, vp]),
     "ralf_tlayer_bwd": (i32, [ctypes.POINTER(RalfTLayerBwdDesc), vp]),
+    "ralf_rope_axes": (i32, [ctypes.POINTER(RalfRopeDesc), vp]),
+    "ralf_paged_kv_write": (i32, [ctypes.POINTER(RalfPagedKV), i32, vp, vp, i64, i64, i64, i64, vp, i64, vp]),
+    "ralf_paged_kv_read": (i32, [ctypes.POINTER(RalfPagedKV), i32, vp, vp, vp, i64, vp]),
+    "ralf_paged_attention_workspace_bytes": (sz, [ctypes.POINTER(RalfPagedAttnDesc)]),
+    "ralf_paged_attention": (i32, [ctypes.POINTER(RalfPagedAttnDesc), vp, sz, vp]),
+    "ralf_logits_process": (i32, [ctypes.POINTER(RalfLogitsDesc), vp]),
     "ralf_sumsq": (i32, [vp, i64, vp, vp]),
     "ralf_clip_coef": (i32, [vp, f32, vp, vp, vp]),
     "ralf_sumsq_partials": (i32, [vp, i64, vp, vp]),

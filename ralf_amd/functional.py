@@ -1014,6 +1014,34 @@ class ScalePEDropFn(Function):
         return ops.scale_pe_dropout(dy.contiguous(), None, 1, scale, p, rt.seed, call), None, None, None, None
 
 
+class RopeAxesFn(Function):
+    """rotary positions with several axes; the gradient is the rotation by the opposite angles"""
+
+    @staticmethod
+    def forward(ctx, x, pos, freq, axis, adjacent):
+        ctx.save_for_backward(pos, freq, axis)
+        ctx.adjacent = adjacent
+        return ops.rope_axes(x, pos, freq, axis, adjacent=adjacent)
+
+    @staticmethod
+    def backward(ctx, dy):
+        pos, freq, axis = ctx.saved_tensors
+        return ops.rope_axes(dy if dy.stride(-1) == 1 else dy.contiguous(), pos, freq, axis, adjacent=ctx.adjacent, inverse=True), None, None, None, None
+
+
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+
+
+def rope_axes(x, pos, freq, axis, adjacent=False):
+    """ops.rope_axes with a gradient for x.  Refused for a LEAF that requires one while a graph is being captured: if an eager autograd graph of that leaf is still
+    alive, its gradient accumulator belongs to the stream of that time, the captured backward would have to wait on it, and the process ends when the capture does.
+    The gradient of a rotation is ops.rope_axes(dy, ..., inverse=True), which can be captured."""
+    if x.requires_grad and x.is_leaf and torch.is_grad_enabled() and _capturing():
+        raise RuntimeError("rope_axes: the gradient of a leaf inside a graph capture; use ops.rope_axes(dy, ..., inverse=True) there, or pass the leaf without requires_grad")
+    return RopeAxesFn.apply(x, pos, freq, axis, adjacent)
+
+
 class EmbedFn(Function):
     """emb(idx) * sqrt(d) + pe[:S]  (nn.Embedding -> PositionalEncoding1d)."""
 

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -1101,4 +1101,232 @@ def mask_sample(logits, allowed=None, forced=None, mode=0, top_k=1, temperature=
     fp, fl = col(pad_flag_col, torch.uint8)
     _call("ralf_mask_sample_step", _p(logits.contiguous()), _p(allowed), _p(forced), mode, top_k, temperature, _p(seed), call_id, _p(out),
           sp, sl, fp, fl, int(pad_id), B, V, float(top_p), int(row0))
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
+# serving operators: rotary positions, the paged key / value cache, attention over it, history-dependent logits
+# ----------------------------------------------------------------------------------------------
+def _on(device):
+    """the device guard of a call on tensors of `device`: kernels go to ITS current stream, whatever the current device is"""
+    return torch.cuda.device(device)
+
+
+def _need_cuda(what, *tensors):
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        assert t.is_cuda, f"{what}: tensors live on the GPU"
+        assert dev is None or t.device == dev, f"{what}: tensors on {dev} and {t.device}"
+        dev = t.device
+    return dev
+
+
+def _rows3(t, what):
+    """[T, heads, dim] with a contiguous last dim -> (token stride, head stride) in elements"""
+    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what}: [tokens, heads, dim] with a contiguous last dim, got {tuple(t.shape)} with strides {t.stride()}"
+    return t.stride(0), t.stride(1)
+
+
+def rope_table(sections, theta=10000.0, ladder="joint", order="blocks", device=None):
+    """(freq float64 [P], axis int32 [P]) of rope_axes for sections = pairs per position axis, P = sum(sections).
+    ladder "joint": pair j turns by theta ** (-j / P) per position, whichever axis it follows; "axis": every axis has the whole ladder over its own pairs.
+    order "blocks": the axes' pairs one block after the other; "round": dealt in turn (0, 1, 2, 0, 1, ...) as long as an axis has pairs left."""
+    sections = [int(n) for n in sections]
+    assert sections and min(sections) >= 0 and sum(sections) > 0, f"rope_table: sections {sections}"
+    assert ladder in ("joint", "axis") and order in ("blocks", "round"), f"rope_table: ladder {ladder!r}, order {order!r}"
+    if order == "blocks":
+        pairs = [(a, i) for a, n in enumerate(sections) for i in range(n)]
+    else:
+        pairs = [(a, i) for i in range(max(sections)) for a, n in enumerate(sections) if i < n]
+    P = len(pairs)
+    freq = [theta ** (-i / sections[a]) if ladder == "axis" else theta ** (-j / P) for j, (a, i) in enumerate(pairs)]
+    return torch.tensor(freq, dtype=torch.float64, device=device), torch.tensor([a for a, _ in pairs], dtype=torch.int32, device=device)
+
+
+def rope_axes(x, pos, freq, axis, *, adjacent=False, inverse=False, out=None):
+    """rotary positions with several axes (ralf_rope_axes): x [T, H, D] fp32 / bf16 (any token / head strides), pos int64 [A, T], freq float64 [P], axis int32 [P]
+    (rope_table).  The first 2 P dims of every head are turned -- pairs (j, P + j), or (2j, 2j + 1) with adjacent -- by pos[axis[j], t] * freq[j]; the others pass.
+    inverse: the opposite angle.  out: a tensor of x's shape and type, x itself for in place."""
+    from ._abi import RalfRopeDesc
+
+    d = RalfRopeDesc()
+    assert x.dtype in _TORCH2CODE, f"rope_axes: dtype {x.dtype}"
+    d.x_ts, d.x_hs = _rows3(x, "rope_axes")
+    T, H, D = x.shape
+    assert pos.dtype == torch.int64 and pos.dim() == 2 and pos.shape[0] > 0 and pos.shape[1] == T and (pos.stride(1) == 1 or T <= 1), "rope_axes: pos is int64 [axes, tokens]"
+    assert freq.dtype == torch.float64 and axis.dtype == torch.int32 and freq.dim() == axis.dim() == 1 and freq.shape == axis.shape and freq.is_contiguous() and axis.is_contiguous(), \
+        "rope_axes: freq float64 [P] and axis int32 [P]"
+    assert 0 < 2 * freq.numel() <= D, f"rope_axes: {freq.numel()} pairs in a head of {D}"
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    assert out.shape == x.shape and out.dtype == x.dtype, "rope_axes: out has x's shape and type"
+    d.y_ts, d.y_hs = _rows3(out, "rope_axes out")
+    dev = _need_cuda("rope_axes", x, pos, freq, axis, out)
+    if x.numel() == 0:
+        return out
+    d.x, d.y, d.pos, d.freq, d.axis = _p(x), _p(out), _p(pos), _p(freq), _p(axis)
+    d.T, d.H, d.D, d.R, d.A, d.pos_as = T, H, D, 2 * freq.numel(), pos.shape[0], pos.stride(0)
+    d.dtype, d.adjacent, d.inverse = dtype_code(x), int(bool(adjacent)), int(bool(inverse))
+    with _on(dev):
+        _call("ralf_rope_axes", ctypes.byref(d))
+    return out
+
+
+class PagedKV(NamedTuple):
+    """a key / value cache in pages: k, v [pages, heads, page, dim] in fp32, bf16, float8_e4m3fn or int8; the 8-bit stores with k_exp, v_exp uint8
+    [pages, heads, page], the row's power of two 2 ** (byte - 127).  paged_kv_pool allocates one; which page belongs to whom is the caller's page table."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_exp: Optional[torch.Tensor] = None
+    v_exp: Optional[torch.Tensor] = None
+
+
+_STORE2CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2, torch.int8: 3}
+
+
+def paged_kv_pool(n_pages, page, heads, dim, store=torch.bfloat16, device="cuda") -> PagedKV:
+    """a zeroed cache of n_pages pages of `page` tokens; store: torch.float32, bfloat16, float8_e4m3fn or int8"""
+    assert store in _STORE2CODE, f"paged_kv_pool: store {store}"
+    k, v = (torch.zeros(n_pages, heads, page, dim, dtype=torch.uint8 if store.itemsize == 1 else store, device=device).view(store) for _ in range(2))
+    if store.itemsize > 1:
+        return PagedKV(k, v)
+    return PagedKV(k, v, *(torch.zeros(n_pages, heads, page, dtype=torch.uint8, device=device) for _ in range(2)))
+
+
+def _paged(what, pool, table, kv_len, d):
+    """fills a RalfPagedKV and returns the tensors it points into"""
+    k, v, ke, ve = pool
+    assert k.dtype in _STORE2CODE and v.dtype == k.dtype, f"{what}: cache of {k.dtype} / {v.dtype}"
+    assert k.dim() == 4 and k.shape == v.shape and k.is_contiguous() and v.is_contiguous(), f"{what}: cache tensors are contiguous [pages, heads, page, dim]"
+    if k.dtype.itemsize == 1:
+        assert all(e is not None and e.dtype == torch.uint8 and e.shape == k.shape[:3] and e.is_contiguous() for e in (ke, ve)), f"{what}: an 8-bit cache has uint8 exponents [pages, heads, page]"
+    assert table.dtype == torch.int32 and table.dim() == 2 and (table.stride(1) == 1 or table.shape[1] <= 1), f"{what}: the page table is int32 [sequences, pages]"
+    B = table.shape[0]
+    assert kv_len.dtype == torch.int32 and kv_len.shape == (B,) and kv_len.is_contiguous(), f"{what}: kv_len is int32 [sequences]"
+    d.k, d.v, d.k_exp, d.v_exp, d.table, d.kv_len = _p(k), _p(v), _p(ke), _p(ve), _p(table), _p(kv_len)
+    d.n_pages, d.heads, d.page, d.dim = k.shape
+    d.store, d.B, d.max_pages, d.table_ld = _STORE2CODE[k.dtype], B, table.shape[1], max(table.stride(0), table.shape[1])
+    assert B <= 1 or table.stride(0) >= table.shape[1], f"{what}: the page table's rows overlap"
+    return k, v, ke, ve, table, kv_len
+
+
+def _starts(t, B, what):
+    assert t.dtype == torch.int32 and t.shape == (B + 1,) and t.is_contiguous(), f"{what}: int32 [sequences + 1], ascending from 0"
+
+
+def paged_kv_write(pool, k, v, table, q_start, kv_len):
+    """the newest tokens of every sequence into the cache, quantised on the way where it holds 8 bits (ralf_paged_kv_write): k, v [T, heads, dim] (any token / head
+    strides of multiples of 8), rows q_start[b] .. q_start[b + 1] - 1 = positions kv_len[b] - n .. kv_len[b] - 1.  kv_len counts them already.  table int32
+    [B, pages per sequence]: a page being written belongs to one sequence.  Rows behind q_start[B] are not stored."""
+    from ._abi import RalfPagedKV
+
+    d = RalfPagedKV()
+    held = _paged("paged_kv_write", pool, table, kv_len, d)
+    _starts(q_start, d.B, "paged_kv_write: q_start")
+    assert k.dtype in _TORCH2CODE and v.dtype == k.dtype and k.shape == v.shape, f"paged_kv_write: k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}"
+    ks, vs = _rows3(k, "paged_kv_write k"), _rows3(v, "paged_kv_write v")
+    assert tuple(k.shape[1:]) == (d.heads, d.dim), f"paged_kv_write: rows of {tuple(k.shape[1:])} for a cache of {(d.heads, d.dim)}"
+    dev = _need_cuda("paged_kv_write", *held, k, v, q_start)
+    with _on(dev):
+        _call("ralf_paged_kv_write", ctypes.byref(d), dtype_code(k), _p(k), _p(v), *ks, *vs, _p(q_start), k.shape[0])
+
+
+def paged_kv_read(pool, table, kv_len, start, rows, dtype=None, out=None):
+    """the cached tokens of every sequence one behind the other, as values (ralf_paged_kv_read) -> (k, v) [rows, heads, dim] of `dtype` (fp32 / bf16): rows start[b] ..
+    start[b + 1] - 1 = positions 0 .. of sequence b, zeros behind kv_len[b].  rows: the host's start[B].  out = (k, v): rows behind start[B] stay as they are
+    (without out they are not initialised)."""
+    from ._abi import RalfPagedKV
+
+    d = RalfPagedKV()
+    held = _paged("paged_kv_read", pool, table, kv_len, d)
+    _starts(start, d.B, "paged_kv_read: start")
+    if out is None:
+        dtype = dtype or (pool.k.dtype if pool.k.dtype in _TORCH2CODE else torch.bfloat16)
+        assert dtype in _TORCH2CODE, f"paged_kv_read: dtype {dtype}"
+        out = tuple(torch.empty(rows, d.heads, d.dim, dtype=dtype, device=pool.k.device) for _ in range(2))
+    k, v = out
+    assert k.dtype in _TORCH2CODE and v.dtype == k.dtype and k.shape == v.shape == (rows, d.heads, d.dim) and k.is_contiguous() and v.is_contiguous(), "paged_kv_read: out is contiguous [rows, heads, dim]"
+    dev = _need_cuda("paged_kv_read", *held, start, k, v)
+    with _on(dev):
+        _call("ralf_paged_kv_read", ctypes.byref(d), dtype_code(k), _p(k), _p(v), _p(start), int(rows))
+    return k, v
+
+
+def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True, window=0, max_q=None, max_kv=None, out=None):
+    """attention of every sequence's newest tokens over its pages (ralf_paged_attention) -> [T, q_heads, dim]: q [T, q_heads, dim], rows as in paged_kv_write (call it
+    first: a token sees its own key); q_heads a multiple of the cache's heads.  causal: position p sees keys <= p; window > 0: only the last `window` of them.
+    q bf16 reads caches of bf16 and 8 bits, q fp32 those of fp32 and 8 bits.  A row without a key gives zeros.  max_q / max_kv: the host's upper bounds of the
+    new tokens and of kv_len of one sequence; they steer how the work is split (a captured graph keeps its split), not what is computed.
+    Rows behind q_start[B] are not written."""
+    from ._abi import RalfPagedAttnDesc
+
+    d = RalfPagedAttnDesc()
+    held = _paged("paged_attention", pool, table, kv_len, d.kv)
+    _starts(q_start, d.kv.B, "paged_attention: q_start")
+    assert q.dtype in _TORCH2CODE, f"paged_attention: dtype {q.dtype}"
+    assert pool.k.dtype.itemsize == 1 or pool.k.dtype == q.dtype, f"paged_attention: queries of {q.dtype} on a cache of {pool.k.dtype}"
+    d.q_ts, d.q_hs = _rows3(q, "paged_attention q")
+    T, Hq, D = q.shape
+    assert D == d.kv.dim and Hq > 0 and Hq % d.kv.heads == 0, f"paged_attention: {Hq} heads of {D} on {d.kv.heads} of {d.kv.dim}"
+    assert window >= 0 and (max_q is None or max_q >= 0) and (max_kv is None or max_kv >= 0), "paged_attention: negative window or bound"
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    assert out.shape == q.shape and out.dtype == q.dtype, "paged_attention: out has q's shape and type"
+    d.o_ts, d.o_hs = _rows3(out, "paged_attention out")
+    dev = _need_cuda("paged_attention", *held, q, q_start, out)
+    d.q, d.o, d.q_start, d.T, d.q_heads, d.dtype = _p(q), _p(out), _p(q_start), T, Hq, dtype_code(q)
+    d.causal, d.window, d.max_q, d.max_kv = int(bool(causal)), min(int(window), 2 ** 31 - 1), min(int(max_q or 0), 2 ** 31 - 1), min(int(max_kv or 0), 2 ** 31 - 1)
+    d.scale = D ** -0.5 if scale is None else float(scale)
+    with _on(dev):
+        need = _lib.lib().ralf_paged_attention_workspace_bytes(ctypes.byref(d))
+        # (a tensor of this call's own: it follows the stream, and a captured graph keeps it to itself)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _call("ralf_paged_attention", ctypes.byref(d), _p(ws), need)
+    return out
+
+
+def logits_process(logits, tokens=None, lens=None, *, prompt_lens=None, repetition=None, presence=None, frequency=None, bias=None, mask=None, mask_row=None, out=None):
+    """penalties for repeated tokens, biases and grammar masks in front of mask_sample (ralf_logits_process) -> logits' shape and type; out=logits works in place.
+    logits [B, V] fp32 / bf16; tokens int64 [B, L] with lens int32 [B] valid ids each (ids outside [0, V) are skipped), the first prompt_lens of them the prompt.
+    repetition float [B] (> 0): x / r or x * r (by sign) for every id in the history; frequency, presence float [B]: x - frequency * count - presence for ids
+    behind the prompt; bias float [V] or [B, V]: added; mask int32 [M, >= ceil(V / 32)], bit v & 31 of word v >> 5: 0 = -inf; mask_row int32 [B]: the row's mask,
+    a value outside [0, M) = none (without mask_row: mask b for row b)."""
+    from ._abi import RalfLogitsDesc
+
+    d = RalfLogitsDesc()
+    assert logits.dtype in _TORCH2CODE and logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits_process: logits are fp32 / bf16 [rows, vocabulary]"
+    B, V = logits.shape
+    assert V > 0, "logits_process: empty vocabulary"
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        assert t is None or (t.dtype == torch.float32 and t.shape == (B,) and t.is_contiguous()), f"logits_process: {name} is float32 [rows]"
+    for name, t in (("lens", lens), ("prompt_lens", prompt_lens), ("mask_row", mask_row)):
+        assert t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"logits_process: {name} is int32 [rows]"
+    if any(t is not None for t in (repetition, presence, frequency)):
+        assert tokens is not None and lens is not None, "logits_process: penalties need tokens and lens"
+    if tokens is not None:
+        assert tokens.dtype == torch.int64 and tokens.dim() == 2 and tokens.shape[0] == B and (tokens.stride(1) == 1 or tokens.shape[1] <= 1), "logits_process: tokens are int64 [rows, history]"
+        d.L, d.tok_ld = tokens.shape[1], max(tokens.stride(0), tokens.shape[1])
+        assert B <= 1 or tokens.stride(0) >= tokens.shape[1], "logits_process: the history's rows overlap"
+    if bias is not None:
+        assert bias.dtype == torch.float32 and tuple(bias.shape) in ((V,), (B, V)) and (bias.stride(-1) == 1 or V == 1), "logits_process: bias is float32 [vocabulary] or [rows, vocabulary]"
+        d.bias_ld = bias.stride(0) if bias.dim() == 2 else 0
+    if mask is not None:
+        assert mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[1] >= (V + 31) // 32 and (mask.stride(1) == 1 or mask.shape[1] == 1), "logits_process: mask is int32 [masks, words of 32 ids]"
+        assert mask_row is not None or mask.shape[0] == B, "logits_process: a mask for every row, or mask_row"
+        d.mask_rows, d.mask_ld = mask.shape[0], max(mask.stride(0), mask.shape[1])
+        assert mask.shape[0] <= 1 or mask.stride(0) >= mask.shape[1], "logits_process: the masks overlap"
+    else:
+        assert mask_row is None, "logits_process: mask_row without masks"
+    if out is None:
+        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
+    assert out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V == 1), "logits_process: out has logits' shape and type"
+    dev = _need_cuda("logits_process", logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask, mask_row, out)
+    d.logits, d.out, d.tokens, d.len, d.prompt_len = _p(logits), _p(out), _p(tokens), _p(lens), _p(prompt_lens)
+    d.repetition, d.presence, d.frequency, d.bias, d.mask, d.mask_row = _p(repetition), _p(presence), _p(frequency), _p(bias), _p(mask), _p(mask_row)
+    d.ld_in, d.ld_out, d.B, d.V, d.dtype = max(logits.stride(0), V), max(out.stride(0), V), B, V, dtype_code(logits)
+    assert B <= 1 or (logits.stride(0) >= V and out.stride(0) >= V), "logits_process: rows overlap"
+    with _on(dev):
+        _call("ralf_logits_process", ctypes.byref(d))
     return out
