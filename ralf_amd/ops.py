@@ -1107,26 +1107,41 @@ def mask_sample(logits, allowed=None, forced=None, mode=0, top_k=1, temperature=
 # ----------------------------------------------------------------------------------------------
 # serving operators: rotary positions, the paged key / value cache, attention over it, history-dependent logits
 # ----------------------------------------------------------------------------------------------
-def _on(device):
-    """the device guard of a call on tensors of `device`: kernels go to ITS current stream, whatever the current device is"""
-    return torch.cuda.device(device)
+# (a decode step is a chain of such calls of a few microseconds each: the checks read every tensor's properties once, a descriptor is filled by position, and the device
+#  and stream are asked for as plain numbers)
+from ._abi import RalfLogitsDesc, RalfPagedAttnDesc, RalfPagedKV, RalfRopeDesc  # noqa: E402
 
 
-def _need_cuda(what, *tensors):
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        assert t.is_cuda, f"{what}: tensors live on the GPU"
-        assert dev is None or t.device == dev, f"{what}: tensors on {dev} and {t.device}"
-        dev = t.device
+def _serve(name, dev, *args):
+    """one C entry on the current stream of device `dev`, whatever the current device is"""
+    fn = getattr(_lib.lib(), name)
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _one_device(what, first, *others):
+    """the index of the device that all tensors (None left out) are on"""
+    dev = first.get_device()
+    assert dev >= 0, f"{what}: tensors live on the GPU"
+    for t in others:
+        assert t is None or t.get_device() == dev, f"{what}: tensors on {first.device} and {t.device}"
     return dev
 
 
 def _rows3(t, what):
-    """[T, heads, dim] with a contiguous last dim -> (token stride, head stride) in elements"""
-    assert t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what}: [tokens, heads, dim] with a contiguous last dim, got {tuple(t.shape)} with strides {t.stride()}"
-    return t.stride(0), t.stride(1)
+    """[T, heads, dim] with a contiguous last dim -> its strides in elements"""
+    st = t.stride()
+    assert len(st) == 3 and (st[2] == 1 or t.shape[2] == 1), f"{what}: [tokens, heads, dim] with a contiguous last dim, got {tuple(t.shape)} with strides {st}"
+    return st
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def rope_table(sections, theta=10000.0, ladder="joint", order="blocks", device=None):
@@ -1149,28 +1164,27 @@ def rope_axes(x, pos, freq, axis, *, adjacent=False, inverse=False, out=None):
     """rotary positions with several axes (ralf_rope_axes): x [T, H, D] fp32 / bf16 (any token / head strides), pos int64 [A, T], freq float64 [P], axis int32 [P]
     (rope_table).  The first 2 P dims of every head are turned -- pairs (j, P + j), or (2j, 2j + 1) with adjacent -- by pos[axis[j], t] * freq[j]; the others pass.
     inverse: the opposite angle.  out: a tensor of x's shape and type, x itself for in place."""
-    from ._abi import RalfRopeDesc
-
-    d = RalfRopeDesc()
-    assert x.dtype in _TORCH2CODE, f"rope_axes: dtype {x.dtype}"
-    d.x_ts, d.x_hs = _rows3(x, "rope_axes")
+    dt = _TORCH2CODE.get(x.dtype)
+    assert dt is not None, f"rope_axes: dtype {x.dtype}"
+    xs = _rows3(x, "rope_axes")
     T, H, D = x.shape
-    assert pos.dtype == torch.int64 and pos.dim() == 2 and pos.shape[0] > 0 and pos.shape[1] == T and (pos.stride(1) == 1 or T <= 1), "rope_axes: pos is int64 [axes, tokens]"
-    assert freq.dtype == torch.float64 and axis.dtype == torch.int32 and freq.dim() == axis.dim() == 1 and freq.shape == axis.shape and freq.is_contiguous() and axis.is_contiguous(), \
+    ps = pos.stride()
+    assert pos.dtype is torch.int64 and len(ps) == 2 and pos.shape[1] == T and pos.shape[0] > 0 and (ps[1] == 1 or T <= 1), "rope_axes: pos is int64 [axes, tokens]"
+    assert freq.dtype is torch.float64 and axis.dtype is torch.int32 and freq.dim() == 1 and freq.shape == axis.shape and freq.is_contiguous() and axis.is_contiguous(), \
         "rope_axes: freq float64 [P] and axis int32 [P]"
-    assert 0 < 2 * freq.numel() <= D, f"rope_axes: {freq.numel()} pairs in a head of {D}"
+    P = freq.shape[0]
+    assert 0 < 2 * P <= D, f"rope_axes: {P} pairs in a head of {D}"
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    assert out.shape == x.shape and out.dtype == x.dtype, "rope_axes: out has x's shape and type"
-    d.y_ts, d.y_hs = _rows3(out, "rope_axes out")
-    dev = _need_cuda("rope_axes", x, pos, freq, axis, out)
-    if x.numel() == 0:
+        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+        ys = (H * D, D)
+    else:
+        assert out.shape == x.shape and out.dtype is x.dtype, "rope_axes: out has x's shape and type"
+        ys = _rows3(out, "rope_axes out")
+    dev = _one_device("rope_axes", x, pos, freq, axis, out)
+    if T * H == 0:
         return out
-    d.x, d.y, d.pos, d.freq, d.axis = _p(x), _p(out), _p(pos), _p(freq), _p(axis)
-    d.T, d.H, d.D, d.R, d.A, d.pos_as = T, H, D, 2 * freq.numel(), pos.shape[0], pos.stride(0)
-    d.dtype, d.adjacent, d.inverse = dtype_code(x), int(bool(adjacent)), int(bool(inverse))
-    with _on(dev):
-        _call("ralf_rope_axes", ctypes.byref(d))
+    d = RalfRopeDesc(x.data_ptr(), out.data_ptr(), pos.data_ptr(), freq.data_ptr(), axis.data_ptr(), T, xs[0], xs[1], ys[0], ys[1], ps[0], H, D, 2 * P, pos.shape[0], dt, adjacent, inverse)
+    _serve("ralf_rope_axes", dev, ctypes.byref(d))
     return out
 
 
@@ -1195,63 +1209,66 @@ def paged_kv_pool(n_pages, page, heads, dim, store=torch.bfloat16, device="cuda"
     return PagedKV(k, v, *(torch.zeros(n_pages, heads, page, dtype=torch.uint8, device=device) for _ in range(2)))
 
 
-def _paged(what, pool, table, kv_len, d):
-    """fills a RalfPagedKV and returns the tensors it points into"""
+def _paged(what, pool, table, kv_len):
+    """the checked RalfPagedKV of a cache, its page table and lengths, and their device"""
     k, v, ke, ve = pool
-    assert k.dtype in _STORE2CODE and v.dtype == k.dtype, f"{what}: cache of {k.dtype} / {v.dtype}"
-    assert k.dim() == 4 and k.shape == v.shape and k.is_contiguous() and v.is_contiguous(), f"{what}: cache tensors are contiguous [pages, heads, page, dim]"
-    if k.dtype.itemsize == 1:
-        assert all(e is not None and e.dtype == torch.uint8 and e.shape == k.shape[:3] and e.is_contiguous() for e in (ke, ve)), f"{what}: an 8-bit cache has uint8 exponents [pages, heads, page]"
-    assert table.dtype == torch.int32 and table.dim() == 2 and (table.stride(1) == 1 or table.shape[1] <= 1), f"{what}: the page table is int32 [sequences, pages]"
-    B = table.shape[0]
-    assert kv_len.dtype == torch.int32 and kv_len.shape == (B,) and kv_len.is_contiguous(), f"{what}: kv_len is int32 [sequences]"
-    d.k, d.v, d.k_exp, d.v_exp, d.table, d.kv_len = _p(k), _p(v), _p(ke), _p(ve), _p(table), _p(kv_len)
-    d.n_pages, d.heads, d.page, d.dim = k.shape
-    d.store, d.B, d.max_pages, d.table_ld = _STORE2CODE[k.dtype], B, table.shape[1], max(table.stride(0), table.shape[1])
-    assert B <= 1 or table.stride(0) >= table.shape[1], f"{what}: the page table's rows overlap"
-    return k, v, ke, ve, table, kv_len
+    store = _STORE2CODE.get(k.dtype)
+    assert store is not None and v.dtype is k.dtype, f"{what}: cache of {k.dtype} / {v.dtype}"
+    shape = k.shape
+    assert len(shape) == 4 and v.shape == shape and k.is_contiguous() and v.is_contiguous(), f"{what}: cache tensors are contiguous [pages, heads, page, dim]"
+    if store >= 2:
+        for e in (ke, ve):
+            assert e is not None and e.dtype is torch.uint8 and e.shape == shape[:3] and e.is_contiguous(), f"{what}: an 8-bit cache has uint8 exponents [pages, heads, page]"
+    else:
+        ke = ve = None
+    ts = table.stride()
+    assert table.dtype is torch.int32 and len(ts) == 2 and (ts[1] == 1 or table.shape[1] <= 1), f"{what}: the page table is int32 [sequences, pages]"
+    B, P = table.shape
+    assert B <= 1 or ts[0] >= P, f"{what}: the page table's rows overlap"
+    assert kv_len.dtype is torch.int32 and kv_len.shape == (B,) and kv_len.is_contiguous(), f"{what}: kv_len is int32 [sequences]"
+    return (RalfPagedKV(k.data_ptr(), v.data_ptr(), _ptr(ke), _ptr(ve), table.data_ptr(), kv_len.data_ptr(), shape[0], max(ts[0], P), shape[2], shape[1], shape[3], store, B, P),
+            (k, v, ke, ve, table, kv_len))
 
 
 def _starts(t, B, what):
-    assert t.dtype == torch.int32 and t.shape == (B + 1,) and t.is_contiguous(), f"{what}: int32 [sequences + 1], ascending from 0"
+    assert t.dtype is torch.int32 and t.shape == (B + 1,) and t.is_contiguous(), f"{what}: int32 [sequences + 1], ascending from 0"
 
 
 def paged_kv_write(pool, k, v, table, q_start, kv_len):
     """the newest tokens of every sequence into the cache, quantised on the way where it holds 8 bits (ralf_paged_kv_write): k, v [T, heads, dim] (any token / head
     strides of multiples of 8), rows q_start[b] .. q_start[b + 1] - 1 = positions kv_len[b] - n .. kv_len[b] - 1.  kv_len counts them already.  table int32
     [B, pages per sequence]: a page being written belongs to one sequence.  Rows behind q_start[B] are not stored."""
-    from ._abi import RalfPagedKV
-
-    d = RalfPagedKV()
-    held = _paged("paged_kv_write", pool, table, kv_len, d)
+    d, held = _paged("paged_kv_write", pool, table, kv_len)
     _starts(q_start, d.B, "paged_kv_write: q_start")
-    assert k.dtype in _TORCH2CODE and v.dtype == k.dtype and k.shape == v.shape, f"paged_kv_write: k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}"
+    dt = _TORCH2CODE.get(k.dtype)
+    assert dt is not None and v.dtype is k.dtype and k.shape == v.shape, f"paged_kv_write: k {k.dtype} {tuple(k.shape)}, v {v.dtype} {tuple(v.shape)}"
     ks, vs = _rows3(k, "paged_kv_write k"), _rows3(v, "paged_kv_write v")
-    assert tuple(k.shape[1:]) == (d.heads, d.dim), f"paged_kv_write: rows of {tuple(k.shape[1:])} for a cache of {(d.heads, d.dim)}"
-    dev = _need_cuda("paged_kv_write", *held, k, v, q_start)
-    with _on(dev):
-        _call("ralf_paged_kv_write", ctypes.byref(d), dtype_code(k), _p(k), _p(v), *ks, *vs, _p(q_start), k.shape[0])
+    T = k.shape[0]
+    assert k.shape[1] == d.heads and k.shape[2] == d.dim, f"paged_kv_write: rows of {tuple(k.shape[1:])} for a cache of {(d.heads, d.dim)}"
+    dev = _one_device("paged_kv_write", k, v, q_start, *held)
+    _serve("ralf_paged_kv_write", dev, ctypes.byref(d), dt, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1], q_start.data_ptr(), T)
 
 
 def paged_kv_read(pool, table, kv_len, start, rows, dtype=None, out=None):
     """the cached tokens of every sequence one behind the other, as values (ralf_paged_kv_read) -> (k, v) [rows, heads, dim] of `dtype` (fp32 / bf16): rows start[b] ..
     start[b + 1] - 1 = positions 0 .. of sequence b, zeros behind kv_len[b].  rows: the host's start[B].  out = (k, v): rows behind start[B] stay as they are
     (without out they are not initialised)."""
-    from ._abi import RalfPagedKV
-
-    d = RalfPagedKV()
-    held = _paged("paged_kv_read", pool, table, kv_len, d)
+    d, held = _paged("paged_kv_read", pool, table, kv_len)
     _starts(start, d.B, "paged_kv_read: start")
+    shape = (rows, d.heads, d.dim)
     if out is None:
         dtype = dtype or (pool.k.dtype if pool.k.dtype in _TORCH2CODE else torch.bfloat16)
         assert dtype in _TORCH2CODE, f"paged_kv_read: dtype {dtype}"
-        out = tuple(torch.empty(rows, d.heads, d.dim, dtype=dtype, device=pool.k.device) for _ in range(2))
-    k, v = out
-    assert k.dtype in _TORCH2CODE and v.dtype == k.dtype and k.shape == v.shape == (rows, d.heads, d.dim) and k.is_contiguous() and v.is_contiguous(), "paged_kv_read: out is contiguous [rows, heads, dim]"
-    dev = _need_cuda("paged_kv_read", *held, start, k, v)
-    with _on(dev):
-        _call("ralf_paged_kv_read", ctypes.byref(d), dtype_code(k), _p(k), _p(v), _p(start), int(rows))
+        k, v = torch.empty(shape, dtype=dtype, device=pool.k.device), torch.empty(shape, dtype=dtype, device=pool.k.device)
+    else:
+        k, v = out
+        assert k.dtype in _TORCH2CODE and v.dtype is k.dtype and k.shape == v.shape == shape and k.is_contiguous() and v.is_contiguous(), "paged_kv_read: out is contiguous [rows, heads, dim]"
+    dev = _one_device("paged_kv_read", k, v, start, *held)
+    _serve("ralf_paged_kv_read", dev, ctypes.byref(d), _TORCH2CODE[k.dtype], k.data_ptr(), v.data_ptr(), start.data_ptr(), rows)
     return k, v
+
+
+_I32_MAX = 2 ** 31 - 1
 
 
 def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True, window=0, max_q=None, max_kv=None, out=None):
@@ -1260,31 +1277,35 @@ def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True,
     q bf16 reads caches of bf16 and 8 bits, q fp32 those of fp32 and 8 bits.  A row without a key gives zeros.  max_q / max_kv: the host's upper bounds of the
     new tokens and of kv_len of one sequence; they steer how the work is split (a captured graph keeps its split), not what is computed.
     Rows behind q_start[B] are not written."""
-    from ._abi import RalfPagedAttnDesc
-
-    d = RalfPagedAttnDesc()
-    held = _paged("paged_attention", pool, table, kv_len, d.kv)
-    _starts(q_start, d.kv.B, "paged_attention: q_start")
-    assert q.dtype in _TORCH2CODE, f"paged_attention: dtype {q.dtype}"
-    assert pool.k.dtype.itemsize == 1 or pool.k.dtype == q.dtype, f"paged_attention: queries of {q.dtype} on a cache of {pool.k.dtype}"
-    d.q_ts, d.q_hs = _rows3(q, "paged_attention q")
+    kv, held = _paged("paged_attention", pool, table, kv_len)
+    _starts(q_start, kv.B, "paged_attention: q_start")
+    dt = _TORCH2CODE.get(q.dtype)
+    assert dt is not None, f"paged_attention: dtype {q.dtype}"
+    assert kv.store >= 2 or kv.store == dt, f"paged_attention: queries of {q.dtype} on a cache of {pool.k.dtype}"
+    qs = _rows3(q, "paged_attention q")
     T, Hq, D = q.shape
-    assert D == d.kv.dim and Hq > 0 and Hq % d.kv.heads == 0, f"paged_attention: {Hq} heads of {D} on {d.kv.heads} of {d.kv.dim}"
-    assert window >= 0 and (max_q is None or max_q >= 0) and (max_kv is None or max_kv >= 0), "paged_attention: negative window or bound"
+    assert D == kv.dim and Hq > 0 and Hq % kv.heads == 0, f"paged_attention: {Hq} heads of {D} on {kv.heads} of {kv.dim}"
+    max_q, max_kv = max_q or 0, max_kv or 0
+    assert window >= 0 and max_q >= 0 and max_kv >= 0, "paged_attention: negative window or bound"
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    assert out.shape == q.shape and out.dtype == q.dtype, "paged_attention: out has q's shape and type"
-    d.o_ts, d.o_hs = _rows3(out, "paged_attention out")
-    dev = _need_cuda("paged_attention", *held, q, q_start, out)
-    d.q, d.o, d.q_start, d.T, d.q_heads, d.dtype = _p(q), _p(out), _p(q_start), T, Hq, dtype_code(q)
-    d.causal, d.window, d.max_q, d.max_kv = int(bool(causal)), min(int(window), 2 ** 31 - 1), min(int(max_q or 0), 2 ** 31 - 1), min(int(max_kv or 0), 2 ** 31 - 1)
-    d.scale = D ** -0.5 if scale is None else float(scale)
-    with _on(dev):
-        need = _lib.lib().ralf_paged_attention_workspace_bytes(ctypes.byref(d))
-        # (a tensor of this call's own: it follows the stream, and a captured graph keeps it to itself)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _call("ralf_paged_attention", ctypes.byref(d), _p(ws), need)
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        os_ = (Hq * D, D)
+    else:
+        assert out.shape == q.shape and out.dtype is q.dtype, "paged_attention: out has q's shape and type"
+        os_ = _rows3(out, "paged_attention out")
+    dev = _one_device("paged_attention", q, q_start, out, *held)
+    d = RalfPagedAttnDesc(kv, q.data_ptr(), out.data_ptr(), q_start.data_ptr(), T, qs[0], qs[1], os_[0], os_[1], Hq, dt, bool(causal), min(window, _I32_MAX), min(max_q, _I32_MAX),
+                          min(max_kv, _I32_MAX), D ** -0.5 if scale is None else scale)
+    ref = ctypes.byref(d)
+    need = _lib.lib().ralf_paged_attention_workspace_bytes(ref)
+    # (a tensor of this call's own: it follows the stream, and a captured graph keeps it to itself)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _serve("ralf_paged_attention", dev, ref, _ptr(ws), need)
     return out
+
+
+def _per_row(t, dtype, B, name):
+    assert t is None or (t.dtype is dtype and t.shape == (B,) and t.is_contiguous()), f"logits_process: {name} is {dtype} [rows]"
 
 
 def logits_process(logits, tokens=None, lens=None, *, prompt_lens=None, repetition=None, presence=None, frequency=None, bias=None, mask=None, mask_row=None, out=None):
@@ -1293,40 +1314,45 @@ def logits_process(logits, tokens=None, lens=None, *, prompt_lens=None, repetiti
     repetition float [B] (> 0): x / r or x * r (by sign) for every id in the history; frequency, presence float [B]: x - frequency * count - presence for ids
     behind the prompt; bias float [V] or [B, V]: added; mask int32 [M, >= ceil(V / 32)], bit v & 31 of word v >> 5: 0 = -inf; mask_row int32 [B]: the row's mask,
     a value outside [0, M) = none (without mask_row: mask b for row b)."""
-    from ._abi import RalfLogitsDesc
-
-    d = RalfLogitsDesc()
-    assert logits.dtype in _TORCH2CODE and logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits_process: logits are fp32 / bf16 [rows, vocabulary]"
+    dt = _TORCH2CODE.get(logits.dtype)
+    ls = logits.stride()
+    assert dt is not None and len(ls) == 2 and (ls[1] == 1 or logits.shape[1] == 1), "logits_process: logits are fp32 / bf16 [rows, vocabulary]"
     B, V = logits.shape
     assert V > 0, "logits_process: empty vocabulary"
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        assert t is None or (t.dtype == torch.float32 and t.shape == (B,) and t.is_contiguous()), f"logits_process: {name} is float32 [rows]"
-    for name, t in (("lens", lens), ("prompt_lens", prompt_lens), ("mask_row", mask_row)):
-        assert t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"logits_process: {name} is int32 [rows]"
-    if any(t is not None for t in (repetition, presence, frequency)):
-        assert tokens is not None and lens is not None, "logits_process: penalties need tokens and lens"
+    _per_row(repetition, torch.float32, B, "repetition"), _per_row(presence, torch.float32, B, "presence"), _per_row(frequency, torch.float32, B, "frequency")
+    _per_row(lens, torch.int32, B, "lens"), _per_row(prompt_lens, torch.int32, B, "prompt_lens"), _per_row(mask_row, torch.int32, B, "mask_row")
+    assert (repetition is None and presence is None and frequency is None) or (tokens is not None and lens is not None), "logits_process: penalties need tokens and lens"
+    L = tok_ld = bias_ld = mask_rows = mask_ld = 0
     if tokens is not None:
-        assert tokens.dtype == torch.int64 and tokens.dim() == 2 and tokens.shape[0] == B and (tokens.stride(1) == 1 or tokens.shape[1] <= 1), "logits_process: tokens are int64 [rows, history]"
-        d.L, d.tok_ld = tokens.shape[1], max(tokens.stride(0), tokens.shape[1])
-        assert B <= 1 or tokens.stride(0) >= tokens.shape[1], "logits_process: the history's rows overlap"
+        ts = tokens.stride()
+        assert tokens.dtype is torch.int64 and len(ts) == 2 and tokens.shape[0] == B and (ts[1] == 1 or tokens.shape[1] <= 1), "logits_process: tokens are int64 [rows, history]"
+        L = tokens.shape[1]
+        tok_ld = max(ts[0], L)
+        assert B <= 1 or ts[0] >= L, "logits_process: the history's rows overlap"
     if bias is not None:
-        assert bias.dtype == torch.float32 and tuple(bias.shape) in ((V,), (B, V)) and (bias.stride(-1) == 1 or V == 1), "logits_process: bias is float32 [vocabulary] or [rows, vocabulary]"
-        d.bias_ld = bias.stride(0) if bias.dim() == 2 else 0
+        bs = bias.stride()
+        assert bias.dtype is torch.float32 and (bias.shape == (V,) or bias.shape == (B, V)) and (bs[-1] == 1 or V == 1), "logits_process: bias is float32 [vocabulary] or [rows, vocabulary]"
+        bias_ld = bs[0] if len(bs) == 2 and B > 1 else 0
     if mask is not None:
-        assert mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[1] >= (V + 31) // 32 and (mask.stride(1) == 1 or mask.shape[1] == 1), "logits_process: mask is int32 [masks, words of 32 ids]"
-        assert mask_row is not None or mask.shape[0] == B, "logits_process: a mask for every row, or mask_row"
-        d.mask_rows, d.mask_ld = mask.shape[0], max(mask.stride(0), mask.shape[1])
-        assert mask.shape[0] <= 1 or mask.stride(0) >= mask.shape[1], "logits_process: the masks overlap"
+        ms = mask.stride()
+        assert mask.dtype is torch.int32 and len(ms) == 2 and 32 * mask.shape[1] >= V and (ms[1] == 1 or mask.shape[1] == 1), "logits_process: mask is int32 [masks, words of 32 ids]"
+        mask_rows = mask.shape[0]
+        assert mask_row is not None or mask_rows == B, "logits_process: a mask for every row, or mask_row"
+        mask_ld = max(ms[0], mask.shape[1])
+        assert mask_rows <= 1 or ms[0] >= mask.shape[1], "logits_process: the masks overlap"
     else:
         assert mask_row is None, "logits_process: mask_row without masks"
     if out is None:
-        out = torch.empty(B, V, dtype=logits.dtype, device=logits.device)
-    assert out.shape == logits.shape and out.dtype == logits.dtype and (out.stride(1) == 1 or V == 1), "logits_process: out has logits' shape and type"
-    dev = _need_cuda("logits_process", logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask, mask_row, out)
-    d.logits, d.out, d.tokens, d.len, d.prompt_len = _p(logits), _p(out), _p(tokens), _p(lens), _p(prompt_lens)
-    d.repetition, d.presence, d.frequency, d.bias, d.mask, d.mask_row = _p(repetition), _p(presence), _p(frequency), _p(bias), _p(mask), _p(mask_row)
-    d.ld_in, d.ld_out, d.B, d.V, d.dtype = max(logits.stride(0), V), max(out.stride(0), V), B, V, dtype_code(logits)
-    assert B <= 1 or (logits.stride(0) >= V and out.stride(0) >= V), "logits_process: rows overlap"
-    with _on(dev):
-        _call("ralf_logits_process", ctypes.byref(d))
+        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
+        ld_out = V
+    else:
+        os_ = out.stride()
+        assert out.shape == logits.shape and out.dtype is logits.dtype and (os_[1] == 1 or V == 1), "logits_process: out has logits' shape and type"
+        ld_out = max(os_[0], V)
+        assert B <= 1 or os_[0] >= V, "logits_process: rows overlap"
+    assert B <= 1 or ls[0] >= V, "logits_process: rows overlap"
+    dev = _one_device("logits_process", logits, tokens, lens, prompt_lens, repetition, presence, frequency, bias, mask, mask_row, out)
+    d = RalfLogitsDesc(logits.data_ptr(), out.data_ptr(), _ptr(tokens), _ptr(lens), _ptr(prompt_lens), _ptr(repetition), _ptr(presence), _ptr(frequency), _ptr(bias), _ptr(mask), _ptr(mask_row),
+                       max(ls[0], V), ld_out, tok_ld, bias_ld, mask_ld, B, V, L, mask_rows, dt)
+    _serve("ralf_logits_process", dev, ctypes.byref(d))
     return out
