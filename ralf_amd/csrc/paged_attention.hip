@@ -21,6 +21,8 @@ using namespace paged;
 struct Args {
     RalfPagedAttnDesc d;
     int G, splits, page_log2;
+    int few_rows;       // sequences of at most so many rows go to few_kernel, the others to many_kernel
+    int few_tiles;      // tiles of a sequence in few_kernel's grid where few_rows bounds them; 0: found from q_start
     float qscale;       // scale * log2(e)
     float* part_o;      // [splits][T * q_heads][dim] unnormalised
     float* part_ml;     // [splits][T * q_heads][2] running maximum (log2 units), sum
@@ -39,16 +41,16 @@ __device__ __forceinline__ int behind(int pos, int window) {
 
 // tile w of BM rows: sequence b's tiles start at q_start[b] * G / BM + b, which leaves every sequence room for ceil(n * G / BM) of them
 template <int BM>
-__device__ __forceinline__ Tile find_tile(const Args& a, int w, int lane) {
+__device__ __forceinline__ Tile find_tile(const Args& a, int w, int lane, int per_seq) {
     Tile t;
     const int B = a.d.kv.B, G = a.G;
-    const int c = count_le([&](int i) { return (int64_t)a.d.q_start[i] * G / BM + i; }, B, w, lane);
+    const int c = per_seq ? w / per_seq + 1 : count_le([&](int i) { return (int64_t)a.d.q_start[i] * G / BM + i; }, B, w, lane);
     t.b = c - 1;
     t.ok = false;
     if (c == 0) return t;
     const int64_t s = a.d.q_start[t.b], e0 = a.d.q_start[t.b + 1], e = e0 < a.d.T ? e0 : a.d.T;
     if (s < 0 || e <= s) return t;
-    const int64_t row0 = (w - (s * G / BM + t.b)) * BM, rows = (e - s) * G;
+    const int64_t row0 = (per_seq ? w % per_seq : w - (s * G / BM + t.b)) * BM, rows = (e - s) * G;
     if (row0 >= rows) return t;
     t.row0 = (int)row0;
     t.rows = (int)rows;
@@ -143,8 +145,8 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     const RalfPagedKV& c = a.d.kv;
     const int split = blockIdx.x % a.splits;
     const int hk = (blockIdx.x / a.splits) % c.heads;
-    const Tile t = find_tile<BM>(a, blockIdx.x / a.splits / c.heads, lane);
-    if (!t.ok) return;
+    const Tile t = find_tile<BM>(a, blockIdx.x / a.splits / c.heads, lane, a.few_tiles);
+    if (!t.ok || t.rows > a.few_rows) return;
     const int64_t tok0 = a.d.q_start[t.b];
     const int row = t.row0 + r16;
     const bool live = row < t.rows;
@@ -466,6 +468,319 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// many rows: 32 to a wave, 8 waves (4 at dim 256) share tiles of 64 keys in LDS, each byte from memory once per 256 (128) rows.
+// v_mfma_f32_32x32x16_bf16: a lane owns row (lane & 31) and of every 32 keys the sixteen 8 (i / 4) + 4 (lane / 32) + i % 4.
+//   * a tile's loads are issued a tile ahead into registers and stored to the other LDS buffer behind the products: one barrier a tile.  8-bit codes become
+//     bf16 values there, once for all waves.
+//   * LDS rows of dim elements without padding; 16-byte chunk c of a K row lies at c ^ (key & 7) -- eight lanes reading one chunk of eight keys touch all banks
+//     once -- and of a V row at c ^ 2 (key & 3), for the transposing reads (4 keys x 16 columns to 16 lanes).
+// ------------------------------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+#define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
+
+template <int D>
+struct Many {
+    static constexpr int WAVES = D == 256 ? 4 : 8, BM = 32 * WAVES, KB = 64;
+    static constexpr int TPK = WAVES;                               // threads of a key row
+    static constexpr int EPT = D / TPK, CH = EPT < 8 ? EPT : 8, NCH = EPT / CH;     // a thread's elements, in chunks of CH
+    static constexpr int CPR = D / 8;                               // 16-byte chunks of an LDS row
+    static constexpr int LDS = 2 * 2 * KB * D * 2;                  // bytes: K and V, two buffers
+    static __device__ __forceinline__ int kswz(int key) { return D >= 64 ? key & 7 : (key >> 1) & 3; }
+    static __device__ __forceinline__ int vswz(int key) { return D >= 64 ? 2 * (key & 3) : 2 * (key & 1); }
+};
+
+// CH codes / values of a chunk, bf16 pairs
+template <int STORE, int CH>
+__device__ __forceinline__ void chunk_bf16(const uint32_t (&raw)[STORE == RALF_KV_BF16 ? CH / 2 : CH / 4], uint32_t ex, uint32_t (&w)[CH / 2]) {
+    if constexpr (STORE == RALF_KV_BF16) {
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) w[i] = raw[i];
+    } else {
+        const float sc = exp_value(ex);
+#pragma unroll
+        for (int i = 0; i < CH / 4; ++i) {
+            if constexpr (STORE == RALF_KV_E4M3) {
+                w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], sc, false));
+                w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[i], sc, true));
+            } else {
+                float f[4];
+                codes_f32<STORE>(raw[i], f);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const bf16x2 b = {(bf16)(f[2 * j] * sc), (bf16)(f[2 * j + 1] * sc)};        // (7 significant bits: exact)
+                    w[2 * i + j] = __builtin_bit_cast(uint32_t, b);
+                }
+            }
+        }
+        if (ex == 255u) {
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) w[i] = 0x7fc07fc0u;
+        }
+    }
+}
+
+template <int D, int STORE>
+__global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_kernel(const Args a, int ntiles) {
+    typedef Many<D> M;
+    constexpr int KB = M::KB, ESZ = STORE == RALF_KV_BF16 ? 2 : 1, RW = M::CH * ESZ / 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ int s_odd;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r32 = lane & 31, h = lane >> 5;
+    const RalfPagedKV& c = a.d.kv;
+    // tiles of one key head and split side by side on one XCD (workgroups are dealt to the 8 XCDs in turn): they read the same keys
+    const int nwg = gridDim.x, q8 = nwg >> 3, r8 = nwg & 7, xcd = blockIdx.x & 7;
+    const int vid = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+    const int hk = vid / ntiles / a.splits, split = vid / ntiles % a.splits;
+    const Tile t = find_tile<M::BM>(a, vid % ntiles, lane, 0);
+    if (!t.ok || t.rows <= a.few_rows) return;
+    if (threadIdx.x == 0) s_odd = 0;
+    const int64_t tok0 = a.d.q_start[t.b];
+    const int row = t.row0 + 32 * wave + r32;
+    const bool live = row < t.rows;
+    const int ti = (live ? row : t.row0) / a.G, hq = hk * a.G + (live ? row : t.row0) % a.G;
+    const int pos = t.first + ti;
+    const int hi = !live ? -1 : a.d.causal && pos < t.L - 1 ? pos : t.L - 1;
+    const int lo = behind(pos, a.d.window);
+    struct Range { int kbeg, kend, lo, hi; };
+    auto range = [&](int r0, int n) {     // the keys that some (kbeg .. kend - 1) and that every one (lo .. hi) of n rows from r0 on sees
+        const int last = (r0 + n < t.rows ? r0 + n : t.rows) - 1;
+        const int p0 = t.first + r0 / a.G, p1 = t.first + last / a.G;
+        return Range{behind(p0, a.d.window), a.d.causal && p1 < t.L ? p1 + 1 : t.L, behind(p1, a.d.window), a.d.causal && p0 < t.L - 1 ? p0 : t.L - 1};
+    };
+    const Range all = range(t.row0, M::BM);
+    const int w0 = t.row0 + 32 * wave;
+    const Range own = w0 < t.rows ? range(w0, 32) : Range{0, 0, 0, -1};
+    const int kbeg = all.kbeg, kend = all.kend, wg_lo = all.lo, wg_hi = all.hi, wbeg = own.kbeg, wend = own.kend, full_lo = own.lo, full_hi = own.hi;
+    const int blk0 = kbeg / KB, nblk = kend > kbeg ? (kend + KB - 1) / KB - blk0 : 0;
+    const int per = (nblk + a.splits - 1) / a.splits;
+    const int sb = blk0 + split * per, se = sb + per < blk0 + nblk ? sb + per : blk0 + nblk;
+
+    u32x4 q[D / 16];
+    {
+        const bf16* qp = (const bf16*)a.d.q + (tok0 + ti) * a.d.q_ts + hq * a.d.q_hs + 8 * h;
+        const uint32_t flip = a.qscale < 0.f ? 0x80008000u : 0u;      // (a negative scale goes into the query, so that the largest score has the largest weight)
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+            q[j] = live && a.qscale != 0.f ? *(const u32x4*)(qp + 16 * j) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[j][i] ^= flip;
+        }
+    }
+    const float qs = a.qscale == 0.f ? 1.f : fabsf(a.qscale);          // (a scale of 0 is a query of 0: hidden scores are -inf, and stay so)
+    f32x16 acc[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
+    float m = -__builtin_inff(), l = 0.f;
+
+    const int* table = c.table + (int64_t)t.b * c.table_ld;
+    const int64_t head_rows = (int64_t)c.heads * c.page;
+    const int skey = threadIdx.x / M::TPK, spart = threadIdx.x % M::TPK;        // the key row and part of it that this thread brings in
+    int pg0, pg1, pg2, pg3;     // of the tile's four sixteens: looked up one tile ahead of their loads
+    auto page_of = [&](int blk, int s) {
+        const int k0 = blk * KB + 16 * s;
+        return blk < se && k0 < t.L ? __builtin_amdgcn_readfirstlane(table[k0 >> a.page_log2]) : -1;
+    };
+    auto look = [&](int blk) { pg0 = page_of(blk, 0); pg1 = page_of(blk, 1); pg2 = page_of(blk, 2); pg3 = page_of(blk, 3); };
+    auto there = [&](int pg) { return pg >= 0 && pg < c.n_pages; };
+    uint32_t kr[M::NCH][RW], vr[M::NCH][RW], kex = 127u, vex = 127u, bad, bad_next = 0u;
+    bool gone;                  // this thread's key is not there
+    auto load = [&](int blk) {
+        const uint32_t b = (there(pg0) ? 0u : 1u) | (there(pg1) ? 0u : 2u) | (there(pg2) ? 0u : 4u) | (there(pg3) ? 0u : 8u);
+        bad_next = b;
+        const int s4 = skey >> 4;
+        const int pg = (s4 & 2) ? (s4 & 1) ? pg3 : pg2 : (s4 & 1) ? pg1 : pg0;
+        const int key = blk * KB + skey;
+        const bool ok = !((b >> s4) & 1u);
+        gone = !ok || key >= t.L;
+        const int64_t row = (ok ? pg : 0) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
+#pragma unroll
+        for (int i = 0; i < M::NCH; ++i) {
+            const int64_t at = (row * D + (i * M::TPK + spart) * M::CH) * ESZ;
+            load_words<RW>((const uint8_t*)c.k + at, kr[i], 4);
+            load_words<RW>((const uint8_t*)c.v + at, vr[i], 4);
+        }
+        if constexpr (STORE >= RALF_KV_E4M3) {
+            kex = ((const uint8_t*)c.k_exp)[row];
+            vex = ((const uint8_t*)c.v_exp)[row];
+        }
+    };
+    auto store = [&](int blk, int buf) {
+        uint8_t* kd = lds + buf * (KB * D * 2);
+        uint8_t* vd = lds + (2 + buf) * (KB * D * 2);
+        const bool mixed = blk * KB < wg_lo || blk * KB + KB - 1 > wg_hi || bad_next;     // some row of the workgroup does not see some key of the tile
+#pragma unroll
+        for (int i = 0; i < M::NCH; ++i) {
+            uint32_t kw[M::CH / 2], vw[M::CH / 2];
+            chunk_bf16<STORE, M::CH>(kr[i], kex, kw);
+            chunk_bf16<STORE, M::CH>(vr[i], vex, vw);
+            if (mixed) {
+                // values that are not there: 0.  Infinities and NaN, which 0 * inf would carry to rows that do not see them: taken out, and given to the rows that do
+                // see them when the loop is done
+#pragma unroll
+                for (int x = 0; x < M::CH / 2; ++x) {
+                    if (gone) vw[x] = 0u;
+                    else if (odd_word<RALF_KV_BF16>(vw[x])) { vw[x] = finite_word<RALF_KV_BF16>(vw[x]); s_odd = 1; }
+                }
+            }
+            const int e = (i * M::TPK + spart) * M::CH, ch = e >> 3, off = (e & 7) * 2;
+            uint8_t* kp = kd + skey * (D * 2) + ((ch ^ M::kswz(skey)) << 4) + off;
+            uint8_t* vp = vd + skey * (D * 2) + ((ch ^ M::vswz(skey)) << 4) + off;
+            if constexpr (M::CH == 8) {
+                *(u32x4*)kp = u32x4{kw[0], kw[1], kw[2], kw[3]};
+                *(u32x4*)vp = u32x4{vw[0], vw[1], vw[2], vw[3]};
+            } else {
+                *(u32x2*)kp = u32x2{kw[0], kw[1]};
+                *(u32x2*)vp = u32x2{vw[0], vw[1]};
+            }
+        }
+    };
+    auto compute = [&](int blk, int buf) {
+        const uint8_t* kd = lds + buf * (KB * D * 2);
+        const uint8_t* vd = lds + (2 + buf) * (KB * D * 2);
+        const int key0 = blk * KB;
+        f32x16 st[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
+            const int key = 32 * kt + r32;
+            const uint8_t* kp = kd + key * (D * 2);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                const bf16x8 kf = *(const bf16x8*)(kp + (((2 * j + h) ^ M::kswz(key)) << 4));
+                st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, q[j]), st[kt], 0, 0, 0);
+            }
+        }
+        if (key0 < full_lo || key0 + KB - 1 > full_hi || bad) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int o = 32 * kt + 8 * (i >> 2) + 4 * h + (i & 3);
+                    const bool see = key0 + o >= lo && key0 + o <= hi && !((bad >> (2 * kt + (i >> 3))) & 1u);
+                    st[kt][i] = see ? st[kt][i] : -__builtin_inff();
+                }
+        }
+        float mx = fmaxf(st[0][0], st[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+        float mo = mx;
+        wave::swap32(mx, mo);
+        mx = fmaxf(m, fmaxf(mx, mo));
+        const float base = mx == -__builtin_inff() ? 0.f : mx * qs;
+        if (__any(mx > m)) {
+            const float alpha = m == -__builtin_inff() ? 0.f : exp2f_(m * qs - base);
+            l *= alpha;
+            m = mx;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[i][j] *= alpha;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                bf16x8 pb;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float p = exp2f_(fmaf(st[kt][8 * u + e], qs, -base));
+                    sum += p;
+                    pb[e] = (bf16)p;
+                }
+                const int Ls = lane & 15;
+#pragma unroll
+                for (int ct = 0; ct < D / 32; ++ct) {
+                    bf16x4 v[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int key = 32 * kt + 16 * u + 8 * x + 4 * h + (Ls >> 2), col = 32 * ct + 16 * ((lane >> 4) & 1) + (Ls & 3) * 4;
+                        v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vd + key * (D * 2) + (((col >> 3) ^ M::vswz(key)) << 4) + (col & 7) * 2));
+                    }
+                    acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, acc[ct], 0, 0, 0);
+                }
+            }
+        l += sum;               // (this half's keys only: the two are added at the end)
+    };
+
+    look(sb);
+    if (sb < se) load(sb);
+    __syncthreads();            // (s_odd)
+    if (sb < se) store(sb, 0);
+    look(sb + 1);
+    __syncthreads();
+    for (int blk = sb; blk < se; ++blk) {
+        const int buf = (blk - sb) & 1;
+        bad = bad_next;
+        if (blk + 1 < se) load(blk + 1);
+        look(blk + 2);
+        if (blk * KB < wend && blk * KB + KB > wbeg) compute(blk, buf);         // (not the tiles that none of the wave's rows sees)
+        if (blk + 1 < se) store(blk + 1, buf ^ 1);
+        __syncthreads();
+    }
+
+    {
+        if (s_odd) {            // the values taken out, to the rows that see them
+            for (int key = sb * KB; key < se * KB && key < t.L; ++key) {
+                const int pg = table[key >> a.page_log2];
+                if (pg < 0 || pg >= c.n_pages) continue;
+                const int k0 = key & ~(KB - 1);
+                uint32_t b = 0u;
+                for (int s = 0; s < 4; ++s) {
+                    const int p = k0 + 16 * s < t.L ? table[(k0 + 16 * s) >> a.page_log2] : -1;
+                    b |= p >= 0 && p < c.n_pages ? 0u : 1u;
+                }
+                if (!(k0 < wg_lo || k0 + KB - 1 > wg_hi || b)) continue;        // (a tile that all see kept them)
+                const int64_t at = pg * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
+                const uint8_t* vrow = (const uint8_t*)c.v + at * (D * ESZ);
+                const bool nan = STORE >= RALF_KV_E4M3 && ((const uint8_t*)c.v_exp)[at] == 255u;
+                const bool see = key >= lo && key <= hi;
+#pragma unroll
+                for (int ct = 0; ct < D / 32; ++ct)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = nan ? __builtin_nanf("") : STORE == RALF_KV_INT8 ? 0.f : odd_value<STORE>(vrow, 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3));
+                        if (see) acc[ct][i] += x;
+                        asm volatile("" ::: "memory");      // (one load at a time)
+                    }
+            }
+        }
+    }
+
+    if (!live) return;
+    float lo2 = l;
+    wave::swap32(l, lo2);
+    l += lo2;
+    const float ml2 = m == -__builtin_inff() ? m : m * qs;
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)split * a.d.T + tok0 + ti) * a.d.q_heads + hq;
+#pragma unroll
+        for (int ct = 0; ct < D / 32; ++ct)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(f32x4*)(a.part_o + at * D + 32 * ct + 8 * g + 4 * h) = f32x4{acc[ct][4 * g], acc[ct][4 * g + 1], acc[ct][4 * g + 2], acc[ct][4 * g + 3]};
+        if (h == 0) { a.part_ml[at * 2] = ml2; a.part_ml[at * 2 + 1] = l; }
+    } else {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bf16* op = (bf16*)a.d.o + (tok0 + ti) * a.d.o_ts + hq * a.d.o_hs;
+#pragma unroll
+        for (int ct = 0; ct < D / 32; ++ct)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                bf16x4 o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = (bf16)(l == 0.f ? 0.f : acc[ct][4 * g + i] * inv);
+                *(bf16x4*)(op + 32 * ct + 8 * g + 4 * h) = o;
+            }
+    }
+}
+
 // the splits of a row joined: a workgroup to a row, its waves take splits in turn
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
@@ -511,42 +826,79 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     else ((bf16*)a.d.o)[at] = (bf16)x;
 }
 
-inline int64_t few_tiles(const RalfPagedAttnDesc& d) { return d.T * (d.q_heads / d.kv.heads) / 16 + d.kv.B; }
-// Workgroups of a key axis: as many as give each CU several (their lengths differ), of 256 keys at least, and no more than the join reads quickly
-inline int splits_for(const RalfPagedAttnDesc& d) {
+// How a call is laid out.  A sequence of more than FEW rows under a key head goes to many_kernel: few_kernel reads the keys again for every 16 rows, a tile of
+// many_kernel costs the same whether it holds 32 rows or 256.
+constexpr int FEW = 64;
+struct Plan {
+    int splits, few_rows, few_tiles;
+    int64_t few_grid, many_tiles;       // tiles of 16 and of 256 (128) rows; 0: the kernel is not launched
+};
+inline Plan plan_for(const RalfPagedAttnDesc& d) {
+    Plan p = {};
+    const int64_t G = d.q_heads / d.kv.heads, B = d.kv.B, rows = d.T * G, heads = d.kv.heads;
+    const int64_t most_rows = d.max_q > 0 && d.max_q < d.T ? d.max_q * G : rows;       // (a wrong bound costs time only: each kernel alone takes every sequence)
+    int64_t wgs = 0, slots = 256;
+    const int bm = d.kv.dim == 256 ? 128 : 256;
+    if (d.dtype == RALF_F32 || most_rows <= FEW) {
+        p.few_rows = 0x7fffffff;
+        p.few_grid = rows / 16 + B;
+        wgs = (p.few_grid < d.T * ((G + 15) / 16) ? p.few_grid : d.T * ((G + 15) / 16)) * heads;
+        slots = 2048;
+    } else {
+        p.many_tiles = rows / bm + B;
+        if (B > 1) {
+            p.few_rows = FEW;
+            p.few_tiles = FEW / 16;
+            p.few_grid = B * (FEW / 16);
+        }
+        wgs = (rows + bm - 1) / bm * heads;
+        slots = 512;
+    }
     int64_t keys = (int64_t)d.kv.max_pages * d.kv.page;
     if (d.max_kv > 0 && d.max_kv < keys) keys = d.max_kv;
-    const int64_t tiles = few_tiles(d) < d.T ? few_tiles(d) : d.T;
-    const int64_t wgs = tiles * d.kv.heads;
-    int64_t s = (2048 + wgs - 1) / wgs;
+    // workgroups along the keys: as many as give each CU several (their lengths differ), of 256 keys at least, and no more than the join reads quickly
+    int64_t s = slots / (wgs > 0 ? wgs : 1);
+    if (slots == 2048) s = (slots + wgs - 1) / wgs;
     const int64_t most = (keys + 255) / 256;
     s = s > most ? most : s;
     s = s > 128 ? 128 : s;
-    return (int)(s < 1 ? 1 : s);
+    p.splits = (int)(s < 1 ? 1 : s);
+    return p;
 }
 
 template <int D, int STORE, bool F32>
-int launch(const Args& a, void* stream) {
-    const int64_t grid = few_tiles(a.d) * a.d.kv.heads * a.splits;
-    RALF_REQUIRE(grid < ((int64_t)1 << 31), "paged_attention: too many tiles");
-    const size_t lds = 4 * 16 * D * sizeof(float);
-    few_kernel<D, STORE, F32><<<(int)grid, 256, lds, (hipStream_t)stream>>>(a);
-    int rc = ralf::check_launch("paged_attention");
-    if (rc || a.splits == 1) return rc;
-    const int64_t R = a.d.T * a.d.q_heads;
-    join_kernel<D, F32><<<(int)R, 256, 0, (hipStream_t)stream>>>(a);
+int launch(const Args& a, const Plan& p, void* stream) {
+    const int64_t heads = a.d.kv.heads;
+    RALF_REQUIRE(p.few_grid * heads * a.splits < ((int64_t)1 << 31) && p.many_tiles * heads * a.splits < ((int64_t)1 << 31), "paged_attention: too many tiles");
+    hipStream_t st = (hipStream_t)stream;
+    if constexpr (!F32) {
+        if (p.many_tiles) {
+            constexpr int lds = Many<D>::LDS;
+            if (lds >= 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(many_kernel<D, STORE>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            many_kernel<D, STORE><<<(int)(p.many_tiles * heads * a.splits), 64 * Many<D>::WAVES, lds, st>>>(a, (int)p.many_tiles);
+            const int rc = ralf::check_launch("paged_attention (many rows)");
+            if (rc) return rc;
+        }
+    }
+    if (p.few_grid) {
+        few_kernel<D, STORE, F32><<<(int)(p.few_grid * heads * a.splits), 256, 4 * 16 * D * sizeof(float), st>>>(a);
+        const int rc = ralf::check_launch("paged_attention");
+        if (rc) return rc;
+    }
+    if (a.splits == 1) return RALF_OK;
+    join_kernel<D, F32><<<(int)(a.d.T * a.d.q_heads), 256, 0, st>>>(a);
     return ralf::check_launch("paged_attention (join)");
 }
 template <int D>
-int launch_dim(const Args& a, void* stream) {
+int launch_dim(const Args& a, const Plan& p, void* stream) {
     if (a.d.dtype == RALF_F32) {
-        if (a.d.kv.store == RALF_KV_F32) return launch<D, RALF_KV_F32, true>(a, stream);
-        if (a.d.kv.store == RALF_KV_E4M3) return launch<D, RALF_KV_E4M3, true>(a, stream);
-        return launch<D, RALF_KV_INT8, true>(a, stream);
+        if (a.d.kv.store == RALF_KV_F32) return launch<D, RALF_KV_F32, true>(a, p, stream);
+        if (a.d.kv.store == RALF_KV_E4M3) return launch<D, RALF_KV_E4M3, true>(a, p, stream);
+        return launch<D, RALF_KV_INT8, true>(a, p, stream);
     }
-    if (a.d.kv.store == RALF_KV_BF16) return launch<D, RALF_KV_BF16, false>(a, stream);
-    if (a.d.kv.store == RALF_KV_E4M3) return launch<D, RALF_KV_E4M3, false>(a, stream);
-    return launch<D, RALF_KV_INT8, false>(a, stream);
+    if (a.d.kv.store == RALF_KV_BF16) return launch<D, RALF_KV_BF16, false>(a, p, stream);
+    if (a.d.kv.store == RALF_KV_E4M3) return launch<D, RALF_KV_E4M3, false>(a, p, stream);
+    return launch<D, RALF_KV_INT8, false>(a, p, stream);
 }
 
 int check(const RalfPagedAttnDesc& d) {
@@ -563,7 +915,7 @@ int check(const RalfPagedAttnDesc& d) {
 
 extern "C" size_t ralf_paged_attention_workspace_bytes(const RalfPagedAttnDesc* d) {
     if (!d || check(*d) || d->T == 0 || d->kv.B == 0) return 0;
-    const int s = splits_for(*d);
+    const int s = plan_for(*d).splits;
     return s > 1 ? (size_t)s * d->T * d->q_heads * (d->kv.dim + 2) * sizeof(float) : 0;
 }
 
@@ -580,7 +932,10 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
     Args a;
     a.d = d;
     a.G = d.q_heads / d.kv.heads;
-    a.splits = splits_for(d);
+    const Plan p = plan_for(d);
+    a.splits = p.splits;
+    a.few_rows = p.few_rows;
+    a.few_tiles = p.few_tiles;
     a.page_log2 = __builtin_ctz(d.kv.page);
     if (d.kv.n_pages == 0) a.d.kv.max_pages = 0;        // (no page to look at: every row is empty)
     a.qscale = d.scale * 1.4426950408889634f;
@@ -592,9 +947,9 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
     a.part_o = (float*)workspace;
     a.part_ml = need ? (float*)workspace + (size_t)a.splits * d.T * d.q_heads * d.kv.dim : nullptr;
     switch (d.kv.dim) {
-        case 32: return launch_dim<32>(a, stream);
-        case 64: return launch_dim<64>(a, stream);
-        case 128: return launch_dim<128>(a, stream);
-        default: return launch_dim<256>(a, stream);
+        case 32: return launch_dim<32>(a, p, stream);
+        case 64: return launch_dim<64>(a, p, stream);
+        case 128: return launch_dim<128>(a, p, stream);
+        default: return launch_dim<256>(a, p, stream);
     }
 }
