@@ -9,14 +9,34 @@
 namespace {
 typedef __bf16 bf16;
 constexpr int THREADS = 512;
-constexpr int MAX_TILE = 16384;     // 64 KiB of counters: two workgroups to a CU
-template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+constexpr int MAX_TILE = 8192;      // 32 KiB of counters: four workgroups, 32 waves, to a CU
+// (rows of an odd vocabulary start anywhere: the vectors are of their elements' alignment, which the memory takes at full width)
+template <typename T> struct Piece { static constexpr int N = 16 / sizeof(T); typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
+typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
 
-template <typename T, int VEC>
+template <typename T>
 __global__ __launch_bounds__(THREADS) void logits_kernel(const RalfLogitsDesc d, int tile, int tiles) {
+    typedef typename Piece<T>::V V;
+    constexpr int N = Piece<T>::N, PIECES = MAX_TILE / (THREADS * N);
     extern __shared__ uint32_t cnt[];
     const int b = blockIdx.x / tiles, v0 = (blockIdx.x % tiles) * tile;
     const int n = d.V - v0 < tile ? d.V - v0 : tile;
+    const T* in = (const T*)d.logits + (int64_t)b * d.ld_in + v0;
+    T* out = (T*)d.out + (int64_t)b * d.ld_out + v0;
+    const float* bias = d.bias ? d.bias + (int64_t)b * d.bias_ld + v0 : nullptr;
+    // all of the thread's logits and biases are on their way while the history is counted
+    V x[PIECES];
+    F4 bb[PIECES][N / 4];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        const int i = (k * THREADS + threadIdx.x) * N;
+        if (i + N <= n) {
+            x[k] = *(const V*)(in + i);
+            if (bias)
+#pragma unroll
+                for (int q = 0; q < N / 4; ++q) bb[k][q] = *(const F4*)(bias + i + 4 * q);
+        }
+    }
     const bool hist = d.repetition || d.presence || d.frequency;
     if (hist) {
         for (int i = threadIdx.x; i < n; i += THREADS) cnt[i] = 0u;
@@ -25,6 +45,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const RalfLogitsDesc d,
         len = len < 0 ? 0 : len > d.L ? d.L : len;
         const int plen = d.prompt_len ? d.prompt_len[b] : 0;
         const int64_t* tok = d.tokens + (int64_t)b * d.tok_ld;
+#pragma unroll 4
         for (int i = threadIdx.x; i < len; i += THREADS) {
             const int64_t v = tok[i] - v0;
             if (v >= 0 && v < n) {
@@ -38,38 +59,38 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const RalfLogitsDesc d,
     const int* mask = nullptr;
     if (d.mask) {
         const int mr = d.mask_row ? d.mask_row[b] : b;
-        if (mr >= 0 && mr < d.mask_rows) mask = d.mask + (int64_t)mr * d.mask_ld;
+        if (mr >= 0 && mr < d.mask_rows) mask = d.mask + (int64_t)mr * d.mask_ld + (v0 >> 5);       // (a tile starts on a word)
     }
-    const T* in = (const T*)d.logits + (int64_t)b * d.ld_in + v0;
-    T* out = (T*)d.out + (int64_t)b * d.ld_out + v0;
-    const float* bias = d.bias ? d.bias + (int64_t)b * d.bias_ld + v0 : nullptr;
-    typedef Vec<T, VEC> V;
-    for (int i = threadIdx.x * VEC; i < n; i += THREADS * VEC) {
-        const V x = *(const V*)(in + i);
-        V y;
-        const uint32_t word = mask ? (uint32_t)mask[(v0 + i) >> 5] >> ((v0 + i) & 31) : ~0u;     // (VEC divides 32 and v0 + i: one word holds them all)
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) {
-            float f = (float)x.v[q];
-            if (hist) {
-                const uint32_t c = cnt[i + q];
-                if (c) {
-                    f = f > 0.f ? f / rep : f * rep;
-                    const uint32_t k = c & 0x7fffffffu;
-                    if (k) f = f - frq * (float)k - pre;
-                }
+    auto one = [&](float f, int i, float add, bool allowed) {
+        if (hist) {
+            const uint32_t c = cnt[i];
+            if (c) {
+                f = f > 0.f ? f / rep : f * rep;
+                const uint32_t k = c & 0x7fffffffu;
+                if (k) f = f - frq * (float)k - pre;
             }
-            if (bias) f += bias[i + q];
-            if (!((word >> q) & 1u)) f = -__builtin_inff();
-            y.v[q] = (T)f;
         }
-        *(V*)(out + i) = y;
+        if (bias) f += add;
+        return allowed ? f : -__builtin_inff();
+    };
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+        const int i = (k * THREADS + threadIdx.x) * N;
+        if (i + N <= n) {
+            const uint32_t word = mask ? (uint32_t)mask[i >> 5] >> (i & 31) : ~0u;
+            V y;
+#pragma unroll
+            for (int q = 0; q < N; ++q) y[q] = (T)one((float)x[k][q], i + q, bias ? bb[k][q >> 2][q & 3] : 0.f, (word >> q) & 1u);
+            *(V*)(out + i) = y;
+        } else {
+            for (int q = i; q < n; ++q) out[q] = (T)one((float)in[q], q, bias ? bias[q] : 0.f, mask ? ((uint32_t)mask[q >> 5] >> (q & 31)) & 1u : true);
+        }
     }
 }
 
-template <typename T, int VEC>
+template <typename T>
 int launch(const RalfLogitsDesc& d, void* stream) {
-    // as few tiles to a row as leave the 256 CUs two workgroups each
+    // the widest tile (the history is read once per tile) that leaves the 256 CUs two workgroups each
     int tiles = 512 / d.B;
     const int most = (d.V + 1023) / 1024, least = (d.V + MAX_TILE - 1) / MAX_TILE;
     tiles = tiles > most ? most : tiles;
@@ -78,7 +99,7 @@ int launch(const RalfLogitsDesc& d, void* stream) {
     tile = (tile + 31) & ~31;
     tiles = (d.V + tile - 1) / tile;
     RALF_REQUIRE((int64_t)d.B * tiles < ((int64_t)1 << 31), "logits_process: too many rows");
-    logits_kernel<T, VEC><<<d.B * tiles, THREADS, (size_t)tile * 4, (hipStream_t)stream>>>(d, tile, tiles);
+    logits_kernel<T><<<d.B * tiles, THREADS, (size_t)tile * 4, (hipStream_t)stream>>>(d, tile, tiles);
     return ralf::check_launch("logits_process");
 }
 }  // namespace
@@ -96,9 +117,5 @@ extern "C" int ralf_logits_process(const RalfLogitsDesc* dp, void* stream) {
     RALF_REQUIRE(!d.bias || d.bias_ld == 0 || d.bias_ld >= d.V, "logits_process: bias rows shorter than V");
     RALF_REQUIRE(!d.mask || d.mask_ld >= (d.V + 31) / 32, "logits_process: mask rows shorter than V bits");
     RALF_REQUIRE(!d.mask || d.mask_row || d.mask_rows >= d.B, "logits_process: without mask_row every row needs a mask of its own");
-    const int vec = d.dtype == RALF_BF16 ? 8 : 4;
-    // whole 16-byte pieces, or single elements where a row does not start on one
-    const bool fits = d.V % vec == 0 && d.ld_in % vec == 0 && d.ld_out % vec == 0 && (uintptr_t)d.logits % 16 == 0 && (uintptr_t)d.out % 16 == 0;
-    if (d.dtype == RALF_BF16) return fits ? launch<bf16, 8>(d, stream) : launch<bf16, 1>(d, stream);
-    return fits ? launch<float, 4>(d, stream) : launch<float, 1>(d, stream);
+    return d.dtype == RALF_BF16 ? launch<bf16>(d, stream) : launch<float>(d, stream);
 }
