@@ -7,8 +7,8 @@
 // are the operand of the second as they stand (the matrix instruction's contraction slots are named after the keys the lane holds), row maxima need
 // two exchanges (lanes 16 and 32 apart), and every rescaling is lane-local.
 //   bf16: v_mfma_f32_16x16x32_bf16, keys and values rounded to bf16 already (8-bit codes are exact in it, their powers of two go to the scores and the
-//         probabilities in fp32), probabilities rounded to bf16 (relative 2^-9; the sum is taken before that rounding in fp32).
-//   fp32: v_mfma_f32_16x16x4_f32 throughout.
+//         probabilities in fp32), probabilities rounded to bf16 (half a step: 2^-8; the sum is taken in fp32 before that rounding).
+//   fp32: v_mfma_f32_16x16x4_f32 on an fp32 cache; on 8-bit codes three bf16 products, the query and the probabilities in three bf16 parts (split3).
 // Running maximum and sum of the softmax in fp32; exponentials base 2 with log2(e) folded into the scale.
 //
 // Masks.  A row that has seen no key keeps max = -inf, sum = 0 and gives zeros.  Keys behind kv_len and keys on bad pages are zeroed as they are loaded; a later
@@ -17,6 +17,8 @@
 
 namespace {
 using namespace paged;
+
+constexpr int MAX_SPLITS = 128;
 
 struct Args {
     RalfPagedAttnDesc d;
@@ -31,7 +33,7 @@ struct Args {
 __device__ __forceinline__ float exp2f_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float sum4(float v) { v += __shfl_xor(v, 16); return v + __shfl_xor(v, 32); }
 
-struct Tile { int b, row0, rows, first, L; bool ok; };  // sequence, first row, its rows, the position of its first new token, its keys
+struct Tile { int b, tok0, row0, rows, first, L; bool ok; };  // sequence, its first token's row of q, first row, its rows, the position of its first new token, its keys
 
 // the first key that a row at position pos sees
 __device__ __forceinline__ int behind(int pos, int window) {
@@ -44,19 +46,33 @@ template <int BM>
 __device__ __forceinline__ Tile find_tile(const Args& a, int w, int lane, int per_seq) {
     Tile t;
     const int B = a.d.kv.B, G = a.G;
-    const int c = per_seq ? w / per_seq + 1 : count_le([&](int i) { return (int64_t)a.d.q_start[i] * G / BM + i; }, B, w, lane);
-    t.b = c - 1;
     t.ok = false;
-    if (c == 0) return t;
-    const int64_t s = a.d.q_start[t.b], e0 = a.d.q_start[t.b + 1], e = e0 < a.d.T ? e0 : a.d.T;
+    int64_t s, e0, L;
+    if (B <= 64 && !per_seq) {          // one lane to a sequence: everything in one trip to memory
+        const int i = lane < B ? lane : B - 1;
+        const int s_ = a.d.q_start[i], e_ = a.d.q_start[i + 1], l_ = a.d.kv.kv_len[i];
+        t.b = __popcll(__ballot(lane < B && (int64_t)s_ * G / BM + lane <= w)) - 1;
+        if (t.b < 0) return t;
+        s = __builtin_amdgcn_readlane(s_, t.b);
+        e0 = __builtin_amdgcn_readlane(e_, t.b);
+        L = __builtin_amdgcn_readlane(l_, t.b);
+    } else {
+        t.b = per_seq ? w / per_seq : count_le([&](int i) { return (int64_t)a.d.q_start[i] * G / BM + i; }, B, w, lane) - 1;
+        if (t.b < 0) return t;
+        s = a.d.q_start[t.b];
+        e0 = a.d.q_start[t.b + 1];
+        L = a.d.kv.kv_len[t.b];
+    }
+    const int64_t e = e0 < a.d.T ? e0 : a.d.T;
     if (s < 0 || e <= s) return t;
     const int64_t row0 = (per_seq ? w % per_seq : w - (s * G / BM + t.b)) * BM, rows = (e - s) * G;
     if (row0 >= rows) return t;
     t.row0 = (int)row0;
     t.rows = (int)rows;
-    const int64_t most = (int64_t)a.d.kv.max_pages * a.d.kv.page, L = a.d.kv.kv_len[t.b];
+    const int64_t most = (int64_t)a.d.kv.max_pages * a.d.kv.page;
     t.L = (int)(L < most ? L : most);
     t.first = (int)(L - (e0 - s));
+    t.tok0 = (int)s;
     t.ok = true;
     return t;
 }
@@ -76,7 +92,9 @@ struct Few {
     static constexpr int KW = EPL * ESZ / 4;                        // dwords of each
     static constexpr int VW = CPL * ESZ < 4 ? 1 : CPL * ESZ / 4;    // dwords of a value row's columns
     // keys of a block: enough bytes in flight with two blocks' registers (loaded one ahead) in 256, the scores' exchanges paid for many keys
-    static constexpr int NT = F32 ? (D * ESZ >= 512 ? 1 : 2) : (D * ESZ >= 128 ? 2 : 4);
+    static constexpr bool FP32 = STORE == RALF_KV_F32;              // fp32 products; otherwise bf16 ones, of fp32 queries in three parts
+    static constexpr int PARTS = F32 && !FP32 ? 3 : 1;
+    static constexpr int NT = FP32 ? (D * ESZ >= 512 ? 1 : 2) : (D * ESZ >= 128 ? 2 : 4);
     static constexpr int REGS = NT * (NK * KW + 4 * VW);
     static constexpr bool TWO = REGS <= 80;                         // two blocks' registers
     static constexpr int WAVES = TWO && D < 256 ? 2 : 1;            // waves to a SIMD that the registers have to leave room for
@@ -127,6 +145,27 @@ __device__ __forceinline__ float odd_value(const uint8_t* row, int i) {
     return fabsf(x) < __builtin_inff() ? 0.f : x;
 }
 
+// Eight fp32 values as sums of three bf16 ones, by cutting off: 8 + 8 + 8 significant bits, so nothing is left out (but what falls below the smallest number).  An
+// 8-bit code is exact in bf16, so three bf16 products of 16 cycles each stand for the fp32 product of 32 dims that takes the fp32 instruction 256.
+__device__ __forceinline__ void split3(const float* f, bf16x8 (&part)[3]) {
+    uint32_t w[3][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        w[0][i] = __float_as_uint(f[i]) & 0xffff0000u;
+        const float a = __uint_as_float(w[0][i]);
+        const float r1 = fabsf(a) < __builtin_inff() ? f[i] - a : f[i] != f[i] ? f[i] : 0.f;
+        w[1][i] = __float_as_uint(r1) & 0xffff0000u;
+        w[2][i] = __float_as_uint(r1 - __uint_as_float(w[1][i]));
+    }
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(w[x][2 * i + 1], w[x][2 * i], 0x07060302u);
+        part[x] = __builtin_bit_cast(bf16x8, v);
+    }
+}
+
 template <int D, int STORE, bool F32>
 struct FewBuf {
     typedef Few<D, STORE, F32> S;
@@ -147,7 +186,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     const int hk = (blockIdx.x / a.splits) % c.heads;
     const Tile t = find_tile<BM>(a, blockIdx.x / a.splits / c.heads, lane, a.few_tiles);
     if (!t.ok || t.rows > a.few_rows) return;
-    const int64_t tok0 = a.d.q_start[t.b];
+    const int64_t tok0 = t.tok0;
     const int row = t.row0 + r16;
     const bool live = row < t.rows;
     const int ti = (live ? row : t.row0) / a.G, hq = hk * a.G + (live ? row : t.row0) % a.G;
@@ -166,21 +205,34 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     const int sb = blk0 + split * per, se = sb + per < blk0 + nblk ? sb + per : blk0 + nblk;
 
     const int64_t qoff = (tok0 + ti) * a.d.q_ts + hq * a.d.q_hs;
-    float qf[F32 ? D / 4 : 1];
-    u32x4 qb[F32 ? 1 : D / 32];
+    float qf[S::FP32 ? D / 4 : 1];
+    u32x4 qb[S::PARTS][S::FP32 ? 1 : D / 32];
 #pragma unroll
     for (int j = 0; j < S::NK; ++j) {
         const int64_t at = qoff + (4 * j + kg) * S::EPL;
         if constexpr (F32) {
+            float f[S::EPL];
 #pragma unroll
             for (int i = 0; i < S::EPL / 4; ++i) {
                 const f32x4 v = live ? *(const f32x4*)((const float*)a.d.q + at + 4 * i) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) qf[j * S::EPL + 4 * i + q] = v[q];
+                for (int q = 0; q < 4; ++q) f[4 * i + q] = v[q];
+            }
+            if constexpr (S::FP32) {
+#pragma unroll
+                for (int i = 0; i < S::EPL; ++i) qf[j * S::EPL + i] = f[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::EPL / 8; ++i) {
+                    bf16x8 part[3];
+                    split3(&f[8 * i], part);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) qb[x][j * (S::EPL / 8) + i] = __builtin_bit_cast(u32x4, part[x]);
+                }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < S::EPL / 8; ++i) qb[j * (S::EPL / 8) + i] = live ? *(const u32x4*)((const bf16*)a.d.q + at + 8 * i) : u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < S::EPL / 8; ++i) qb[0][j * (S::EPL / 8) + i] = live ? *(const u32x4*)((const bf16*)a.d.q + at + 8 * i) : u32x4{0u, 0u, 0u, 0u};
         }
     }
 
@@ -233,17 +285,9 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
             f32x4 st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < S::NK; ++j) {
-                if constexpr (F32) {
+                if constexpr (S::FP32) {
 #pragma unroll
-                    for (int x = 0; x < S::KW; ++x) {
-                        if constexpr (STORE == RALF_KV_F32) st = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.k[s][j][x]), qf[j * S::EPL + x], st, 0, 0, 0);
-                        else {
-                            float f[4];
-                            codes_f32<STORE>(w.k[s][j][x], f);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) st = __builtin_amdgcn_mfma_f32_16x16x4f32(f[i], qf[j * S::EPL + 4 * x + i], st, 0, 0, 0);
-                        }
-                    }
+                    for (int x = 0; x < S::KW; ++x) st = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.k[s][j][x]), qf[j * S::EPL + x], st, 0, 0, 0);
                 } else {
 #pragma unroll
                     for (int x = 0; x < S::EPL / 8; ++x) {
@@ -253,7 +297,9 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
                             const u32x2 u = codes_bf16<STORE>(w.k[s][j][2 * x]), v = codes_bf16<STORE>(w.k[s][j][2 * x + 1]);
                             kv = u32x4{u[0], u[1], v[0], v[1]};
                         }
-                        st = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv), __builtin_bit_cast(bf16x8, qb[j * (S::EPL / 8) + x]), st, 0, 0, 0);
+#pragma unroll
+                        for (int y = S::PARTS - 1; y >= 0; --y)
+                            st = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv), __builtin_bit_cast(bf16x8, qb[y][j * (S::EPL / 8) + x]), st, 0, 0, 0);
                     }
                 }
             }
@@ -323,31 +369,19 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
             }
         }
         // values
-        if constexpr (F32) {
+        if constexpr (S::FP32) {
 #pragma unroll
-            for (int e = 0; e < 4 * NT; ++e) {
-                float f[CPL];
-                if constexpr (STORE == RALF_KV_F32) {
+            for (int e = 0; e < 4 * NT; ++e)
 #pragma unroll
-                    for (int q = 0; q < CPL; ++q) f[q] = __uint_as_float(w.v[e][q]);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < S::VW; ++x) {
-                        float g[4];
-                        codes_f32<STORE>(w.v[e][x], g);
-#pragma unroll
-                        for (int i = 0; i < (CPL < 4 ? CPL : 4); ++i) f[4 * x + i] = g[i];
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < CPL; ++q) acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[q], p[e], acc[q], 0, 0, 0);
-            }
+                for (int q = 0; q < CPL; ++q) acc[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.v[e][q]), p[e], acc[q], 0, 0, 0);
         } else {
 #pragma unroll
             for (int g = 0; g < NT / 2; ++g) {
-                bf16x8 pb;
+                bf16x8 pb[S::PARTS];
+                if constexpr (S::PARTS == 3) split3(&p[8 * g], pb);
+                else
 #pragma unroll
-                for (int i = 0; i < 8; ++i) pb[i] = (bf16)p[8 * g + i];
+                    for (int i = 0; i < 8; ++i) pb[0][i] = (bf16)p[8 * g + i];
 #pragma unroll
                 for (int q = 0; q < CPL; q += 2) {
                     // columns q, q + 1 of the lane, keys in the order of pb: pairs of keys side by side
@@ -364,8 +398,11 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
                             v1[e] = u[1];
                         }
                     }
-                    acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v0), pb, acc[q], 0, 0, 0);
-                    acc[q + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v1), pb, acc[q + 1], 0, 0, 0);
+#pragma unroll
+                    for (int y = S::PARTS - 1; y >= 0; --y) {
+                        acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v0), pb[y], acc[q], 0, 0, 0);
+                        acc[q + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v1), pb[y], acc[q + 1], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -537,7 +574,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     const Tile t = find_tile<M::BM>(a, vid % ntiles, lane, 0);
     if (!t.ok || t.rows <= a.few_rows) return;
     if (threadIdx.x == 0) s_odd = 0;
-    const int64_t tok0 = a.d.q_start[t.b];
+    const int64_t tok0 = t.tok0;
     const int row = t.row0 + 32 * wave + r32;
     const bool live = row < t.rows;
     const int ti = (live ? row : t.row0) / a.G, hq = hk * a.G + (live ? row : t.row0) % a.G;
@@ -781,47 +818,44 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     }
 }
 
-// the splits of a row joined: a workgroup to a row, its waves take splits in turn
+// The splits of a row joined, a workgroup to a row: the splits' maxima and sums give each its weight (LDS), then their sums are added up, several splits at once
+// and eight loads of each in flight.
 template <int D, bool F32>
 __global__ __launch_bounds__(256) void join_kernel(const Args a) {
-    constexpr int LANES = D / 4 < 64 ? D / 4 : 64;                  // lanes of a row, 4 columns each
+    constexpr int LANES = D / 4;                                    // threads of a split's row, 4 columns each
     constexpr int WAYS = 256 / LANES;                               // splits at once
-    __shared__ float so[WAYS][D];
-    __shared__ float sf[WAYS];
+    __shared__ float so[WAYS][D], weight[MAX_SPLITS], red[4][2];
     const int64_t R = a.d.T * a.d.q_heads, r = blockIdx.x;
     const int64_t t = r / a.d.q_heads;
     const int h = (int)(r - t * a.d.q_heads);
     if (t < a.d.q_start[0] || t >= a.d.q_start[a.d.kv.B]) return;
-    const int way = threadIdx.x / LANES, ln = threadIdx.x % LANES;
-    float mm = -__builtin_inff(), ll = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = way; s < a.splits; s += WAYS) {
-        const float ms = a.part_ml[((int64_t)s * R + r) * 2], ls = a.part_ml[((int64_t)s * R + r) * 2 + 1];
-        const f32x4 v = *(const f32x4*)(a.part_o + ((int64_t)s * R + r) * D + 4 * ln);
-        const float mn = fmaxf(mm, ms), base = mn == -__builtin_inff() ? 0.f : mn, f0 = exp2f_(mm - base), f1 = exp2f_(ms - base);
-        ll = ll * f0 + ls * f1;
-        o = o * f0 + v * f1;
-        mm = mn;
-    }
-    *(f32x4*)&so[way][4 * ln] = o;
-    __shared__ float sl[WAYS];
-    if (ln == 0) { sf[way] = mm; sl[way] = ll; }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    static_assert(MAX_SPLITS <= 256, "one thread to a split's maximum");
+    const bool have = tid < a.splits;
+    const float ms = have ? a.part_ml[((int64_t)tid * R + r) * 2] : -__builtin_inff(), ls = have ? a.part_ml[((int64_t)tid * R + r) * 2 + 1] : 0.f;
+    const float wm = wave::max64(ms);
+    if (lane == 0) red[wave][0] = wm;
     __syncthreads();
-    if (threadIdx.x >= D) return;
-    mm = sf[0];
-#pragma unroll
-    for (int w = 1; w < WAYS; ++w) mm = fmaxf(mm, sf[w]);
-    const float base = mm == -__builtin_inff() ? 0.f : mm;
+    const float mm = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])), base = mm == -__builtin_inff() ? 0.f : mm;
+    const float f = exp2f_(ms - base);
+    if (have) weight[tid] = f;
+    const float wl = wave::sum64(f * ls);
+    if (lane == 0) red[wave][1] = wl;
+    __syncthreads();
+    const float ll = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
+    const int way = tid / LANES, ln = tid % LANES;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    const float* src = a.part_o + r * D + 4 * ln;
+#pragma unroll 8
+    for (int s = way; s < a.splits; s += WAYS) o += *(const f32x4*)(src + (int64_t)s * R * D) * weight[s];
+    *(f32x4*)&so[way][4 * ln] = o;
+    __syncthreads();
+    if (tid >= D) return;
     float x = 0.f;
-    ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAYS; ++w) {
-        const float f = exp2f_(sf[w] - base);
-        ll += f * sl[w];
-        x += f * so[w][threadIdx.x];
-    }
+    for (int w = 0; w < WAYS; ++w) x += so[w][tid];
     x = ll == 0.f ? 0.f : x / ll;
-    const int64_t at = t * a.d.o_ts + h * a.d.o_hs + threadIdx.x;
+    const int64_t at = t * a.d.o_ts + h * a.d.o_hs + tid;
     if constexpr (F32) ((float*)a.d.o)[at] = x;
     else ((bf16*)a.d.o)[at] = (bf16)x;
 }
@@ -837,31 +871,35 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     Plan p = {};
     const int64_t G = d.q_heads / d.kv.heads, B = d.kv.B, rows = d.T * G, heads = d.kv.heads;
     const int64_t most_rows = d.max_q > 0 && d.max_q < d.T ? d.max_q * G : rows;       // (a wrong bound costs time only: each kernel alone takes every sequence)
-    int64_t wgs = 0, slots = 256;
-    const int bm = d.kv.dim == 256 ? 128 : 256;
+    int64_t keys = (int64_t)d.kv.max_pages * d.kv.page;
+    if (d.max_kv > 0 && d.max_kv < keys) keys = d.max_kv;
+    if (d.causal && d.window > 0 && d.window + 256 < keys) keys = d.window + 256;      // (what a tile can see of them)
+    int64_t s;
     if (d.dtype == RALF_F32 || most_rows <= FEW) {
         p.few_rows = 0x7fffffff;
         p.few_grid = rows / 16 + B;
-        wgs = (p.few_grid < d.T * ((G + 15) / 16) ? p.few_grid : d.T * ((G + 15) / 16)) * heads;
-        slots = 2048;
+        const int64_t tiles = d.T * ((G + 15) / 16), wgs = (p.few_grid < tiles ? p.few_grid : tiles) * heads;
+        // Splits of the keys.  A wave takes `turns` blocks of 32 keys one behind the other; two workgroups to a CU run at once.  Splitting costs the join (5 us, some 6
+        // turns), so short axes stay whole; longer ones are cut until the card is full or a wave has two turns left, and to 16 turns at most, so that sequences of
+        // different lengths even out (64 sequences of 2048 - 8192: 154 us against 162 in one piece).
+        const int64_t turns = (keys + 127) / 128;
+        const int64_t fill = (512 + wgs - 1) / wgs, even = (turns + 15) / 16;
+        s = fill < turns / 2 ? fill : turns / 2;
+        s = turns < 8 ? 1 : s > even ? s : even;
     } else {
+        const int bm = d.kv.dim == 256 ? 128 : 256;
         p.many_tiles = rows / bm + B;
         if (B > 1) {
             p.few_rows = FEW;
             p.few_tiles = FEW / 16;
             p.few_grid = B * (FEW / 16);
         }
-        wgs = (rows + bm - 1) / bm * heads;
-        slots = 512;
+        // one workgroup to a CU: cut the keys only as far as leaves every CU one, in pieces of 4 tiles at least
+        const int64_t wgs = (rows + bm - 1) / bm * heads;
+        s = 256 / wgs;
+        if (s > keys / 256) s = keys / 256;
     }
-    int64_t keys = (int64_t)d.kv.max_pages * d.kv.page;
-    if (d.max_kv > 0 && d.max_kv < keys) keys = d.max_kv;
-    // workgroups along the keys: as many as give each CU several (their lengths differ), of 256 keys at least, and no more than the join reads quickly
-    int64_t s = slots / (wgs > 0 ? wgs : 1);
-    if (slots == 2048) s = (slots + wgs - 1) / wgs;
-    const int64_t most = (keys + 255) / 256;
-    s = s > most ? most : s;
-    s = s > 128 ? 128 : s;
+    s = s > MAX_SPLITS ? MAX_SPLITS : s;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
 }

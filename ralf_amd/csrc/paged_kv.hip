@@ -22,21 +22,24 @@ struct ReadArgs {
     const int* start;
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8], u32x4& raw0, u32x4& raw1) {
-    if constexpr (sizeof(T) == 2) {
-        raw0 = *(const u32x4*)p;
-        raw1 = raw0;
+// 8 elements as loaded -> fp32 (bf16: r0 alone)
+template <typename T> __device__ __forceinline__ void spread(const u32x4 r0, const u32x4 r1, float (&f)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __builtin_bit_cast(float, raw0[i] << 16);
-            f[2 * i + 1] = __builtin_bit_cast(float, raw0[i] & 0xffff0000u);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            f[2 * i] = __uint_as_float(r0[i] << 16);
+            f[2 * i + 1] = __uint_as_float(r0[i] & 0xffff0000u);
+        } else {
+            f[i] = __uint_as_float(r0[i]);
+            f[4 + i] = __uint_as_float(r1[i]);
         }
-    } else {
-        raw0 = *(const u32x4*)p;
-        raw1 = *(const u32x4*)(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(raw0[i]); f[4 + i] = __uint_as_float(raw1[i]); }
     }
+}
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+    const u32x4 r0 = *(const u32x4*)p;
+    u32x4 r1 = r0;
+    if constexpr (sizeof(T) == 4) r1 = *(const u32x4*)(p + 4);
+    spread<T>(r0, r1, f);
 }
 
 // token `t` (the same in all lanes) -> page * (heads * page) .. row index of head 0, or -1 where nothing is to be stored / to be read
@@ -48,54 +51,62 @@ __device__ __forceinline__ int64_t place(const RalfPagedKV& c, int b, int64_t p)
     return (int64_t)pg * c.heads * c.page + (p - (int64_t)pi * c.page);
 }
 
+// one row's share of a lane -> the pool
+template <typename T, int STORE, int LANES, int D>
+__device__ __forceinline__ void store_row(const RalfPagedKV& c, bool isv, int64_t row, int e0, const u32x4 r0, const u32x4 r1) {
+    if constexpr (STORE <= RALF_KV_BF16) {
+        T* dst = (T*)(isv ? c.v : c.k) + row * D + e0;
+        *(u32x4*)dst = r0;
+        if constexpr (sizeof(T) == 4) *(u32x4*)(dst + 4) = r1;
+    } else {
+        float f[8];
+        spread<T>(r0, r1, f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const uint32_t u = __float_as_uint(f[i]) & 0x7fffffffu; m = m > u ? m : u; }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) { const uint32_t u = __shfl_xor(m, o); m = m > u ? m : u; }
+        const uint32_t ex = exp_byte<STORE>(m);
+        u32x2 code = {0u, 0u};
+        if (ex != 255u) {
+            const float inv = exp_inverse(ex);
+            if constexpr (STORE == RALF_KV_E4M3) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, 0, false);
+                    code[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, w, true);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) code[i >> 2] |= ((uint32_t)(int)rintf(f[i] * inv) & 0xffu) << (8 * (i & 3));
+            }
+        }
+        *(u32x2*)((uint8_t*)(isv ? c.v : c.k) + row * D + e0) = code;
+        if (e0 == 0) ((uint8_t*)(isv ? c.v_exp : c.k_exp))[row] = (uint8_t)ex;
+    }
+}
+
 template <int D, typename T, int STORE>
 __global__ __launch_bounds__(256) void write_kernel(const WriteArgs a) {
     constexpr int LANES = D / 8, RI = 64 / LANES;       // lanes of a row, rows at once
     const RalfPagedKV& c = a.c;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, e0 = (lane % LANES) * 8;
     const int64_t nw = (int64_t)gridDim.x * 4;
     for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < a.T; t += nw) {
         const int b = count_le([&](int i) { return (int64_t)a.q_start[i + 1]; }, c.B, t, lane);
         if (b >= c.B) continue;
         const int64_t cell = place(c, b, (int64_t)c.kv_len[b] - a.q_start[b + 1] + t);
         if (cell < 0) continue;
-        const int e0 = (lane % LANES) * 8;
-        for (int r = lane / LANES; r < 2 * c.heads; r += RI) {      // (a whole row is in or out: the exchange below stays within rows)
-            const int h = r < c.heads ? r : r - c.heads;
+        // (a whole row is in or out: the exchange of its largest magnitude stays within rows.  Several rows' loads in flight at once -- 2 or 4 -- measured slower,
+        //  22-24 against 17 us at 10 600 tokens of 2 x 8 x 128: the registers cost more waves than the loads gained)
+        for (int r = lane / LANES; r < 2 * c.heads; r += RI) {
             const bool isv = r >= c.heads;
+            const int h = isv ? r - c.heads : r;
             const T* src = isv ? (const T*)a.v + t * a.v_ts + h * a.v_hs : (const T*)a.k + t * a.k_ts + h * a.k_hs;
-            const int64_t row = cell + (int64_t)h * c.page;
-            float f[8];
-            u32x4 r0, r1;
-            load8(src + e0, f, r0, r1);
-            if constexpr (STORE <= RALF_KV_BF16) {
-                T* dst = (T*)(isv ? c.v : c.k) + row * D + e0;
-                *(u32x4*)dst = r0;
-                if constexpr (sizeof(T) == 4) *(u32x4*)(dst + 4) = r1;
-            } else {
-                uint32_t m = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) { const uint32_t u = __builtin_bit_cast(uint32_t, f[i]) & 0x7fffffffu; m = m > u ? m : u; }
-#pragma unroll
-                for (int o = 1; o < LANES; o <<= 1) { const uint32_t u = __shfl_xor(m, o); m = m > u ? m : u; }
-                const uint32_t ex = exp_byte<STORE>(m);
-                const float inv = ex == 255u ? 0.f : exp_inverse(ex);
-                u32x2 code = {0u, 0u};
-                if (ex != 255u) {
-                    if constexpr (STORE == RALF_KV_E4M3) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, 0, false);
-                            code[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, w, true);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) code[i >> 2] |= ((uint32_t)(int)rintf(f[i] * inv) & 0xffu) << (8 * (i & 3));
-                    }
-                }
-                *(u32x2*)((uint8_t*)(isv ? c.v : c.k) + row * D + e0) = code;
-                if (e0 == 0) ((uint8_t*)(isv ? c.v_exp : c.k_exp))[row] = (uint8_t)ex;
-            }
+            const u32x4 r0 = *(const u32x4*)(src + e0);
+            u32x4 r1 = r0;
+            if constexpr (sizeof(T) == 4) r1 = *(const u32x4*)(src + e0 + 4);
+            store_row<T, STORE, LANES, D>(c, isv, cell + (int64_t)h * c.page, e0, r0, r1);
         }
     }
 }
@@ -118,14 +129,13 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
             const bool isv = r >= c.heads;
             const int64_t row = cell + (int64_t)h * c.page;
             float f[8];
-            u32x4 r0, r1;
             if (cell < 0) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = 0.f;
             } else if constexpr (STORE == RALF_KV_F32) {
-                load8((const float*)(isv ? c.v : c.k) + row * D + e0, f, r0, r1);
+                load8((const float*)(isv ? c.v : c.k) + row * D + e0, f);
             } else if constexpr (STORE == RALF_KV_BF16) {
-                load8((const bf16*)(isv ? c.v : c.k) + row * D + e0, f, r0, r1);
+                load8((const bf16*)(isv ? c.v : c.k) + row * D + e0, f);
             } else {
                 const u32x2 w = *(const u32x2*)((const uint8_t*)(isv ? c.v : c.k) + row * D + e0);
                 const float s = exp_value(((const uint8_t*)(isv ? c.v_exp : c.k_exp))[row]);
