@@ -573,7 +573,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     const int hk = vid / ntiles / a.splits, split = vid / ntiles % a.splits;
     const Tile t = find_tile<M::BM>(a, vid % ntiles, lane, 0);
     if (!t.ok || t.rows <= a.few_rows) return;
-    if (threadIdx.x == 0) s_odd = 0;
+    if (threadIdx.x == 0) s_odd = 0;        // (a barrier ahead of the first value stored)
     const int64_t tok0 = t.tok0;
     const int row = t.row0 + 32 * wave + r32;
     const bool live = row < t.rows;
@@ -590,7 +590,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     const Range all = range(t.row0, M::BM);
     const int w0 = t.row0 + 32 * wave;
     const Range own = w0 < t.rows ? range(w0, 32) : Range{0, 0, 0, -1};
-    const int kbeg = all.kbeg, kend = all.kend, wg_lo = all.lo, wg_hi = all.hi, wbeg = own.kbeg, wend = own.kend, full_lo = own.lo, full_hi = own.hi;
+    const int kbeg = all.kbeg, kend = all.kend, wg_lo = all.lo, wg_hi = all.hi, full_lo = own.lo, full_hi = own.hi;
     const int blk0 = kbeg / KB, nblk = kend > kbeg ? (kend + KB - 1) / KB - blk0 : 0;
     const int per = (nblk + a.splits - 1) / a.splits;
     const int sb = blk0 + split * per, se = sb + per < blk0 + nblk ? sb + per : blk0 + nblk;
@@ -612,155 +612,196 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
-    float m = -__builtin_inff(), l = 0.f;
+    // the reference of the exponentials, in log2 units and always a whole number, so that moving it scales what has been summed up exactly; it follows the largest
+    // score in steps of 8 and more (a weight is then 2^8 at most, which costs fp32 sums and bf16 weights nothing)
+    float m2 = -__builtin_inff(), l = 0.f;
 
     const int* table = c.table + (int64_t)t.b * c.table_ld;
     const int64_t head_rows = (int64_t)c.heads * c.page;
-    const int skey = threadIdx.x / M::TPK, spart = threadIdx.x % M::TPK;        // the key row and part of it that this thread brings in
-    int pg0, pg1, pg2, pg3;     // of the tile's four sixteens: looked up one tile ahead of their loads
-    auto page_of = [&](int blk, int s) {
-        const int k0 = blk * KB + 16 * s;
-        return blk < se && k0 < t.L ? __builtin_amdgcn_readfirstlane(table[k0 >> a.page_log2]) : -1;
-    };
-    auto look = [&](int blk) { pg0 = page_of(blk, 0); pg1 = page_of(blk, 1); pg2 = page_of(blk, 2); pg3 = page_of(blk, 3); };
+    const int skey = threadIdx.x / M::TPK, spart = threadIdx.x % M::TPK, s4 = skey >> 4;        // the key row and part of it that this thread brings in
     auto there = [&](int pg) { return pg >= 0 && pg < c.n_pages; };
-    uint32_t kr[M::NCH][RW], vr[M::NCH][RW], kex = 127u, vex = 127u, bad, bad_next = 0u;
-    bool gone;                  // this thread's key is not there
-    auto load = [&](int blk) {
-        const uint32_t b = (there(pg0) ? 0u : 1u) | (there(pg1) ? 0u : 2u) | (there(pg2) ? 0u : 4u) | (there(pg3) ? 0u : 8u);
-        bad_next = b;
-        const int s4 = skey >> 4;
-        const int pg = (s4 & 2) ? (s4 & 1) ? pg3 : pg2 : (s4 & 1) ? pg1 : pg0;
+    typedef int Pages __attribute__((ext_vector_type(4)));       // of a tile's four sixteens: looked up one tile ahead of their loads
+    auto look = [&](int blk) {
+        auto one = [&](int s) {
+            const int k0 = blk * KB + 16 * s;
+            return blk < se && k0 < t.L ? __builtin_amdgcn_readfirstlane(table[k0 >> a.page_log2]) : -1;
+        };
+        return Pages{one(0), one(1), one(2), one(3)};
+    };
+    auto bad_of = [&](const Pages g) { return (there(g[0]) ? 0u : 1u) | (there(g[1]) ? 0u : 2u) | (there(g[2]) ? 0u : 4u) | (there(g[3]) ? 0u : 8u); };
+    auto row_of = [&](int blk, const Pages g) {        // this thread's key's row of the pool (of page 0 if it is not there), negative - 1 if it is not there
+        const int pg = (s4 & 2) ? (s4 & 1) ? g[3] : g[2] : (s4 & 1) ? g[1] : g[0];
         const int key = blk * KB + skey;
-        const bool ok = !((b >> s4) & 1u);
-        gone = !ok || key >= t.L;
-        const int64_t row = (ok ? pg : 0) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
+        const int64_t row = (there(pg) ? pg : 0) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
+        return there(pg) && key < t.L ? row : -1 - row;
+    };
+    uint32_t kr[M::NCH][RW], vr[M::NCH][RW], kex = 127u, vex = 127u;
+    bool vgone = false;
+    auto load = [&](const void* base, const void* exps, int64_t row, uint32_t (&w)[M::NCH][RW], uint32_t& ex) {
+        row = row < 0 ? -1 - row : row;
+#pragma unroll
+        for (int i = 0; i < M::NCH; ++i) load_words<RW>((const uint8_t*)base + (row * D + (i * M::TPK + spart) * M::CH) * ESZ, w[i], 4);
+        if constexpr (STORE >= RALF_KV_E4M3) ex = ((const uint8_t*)exps)[row];
+    };
+    uint8_t* const ks = lds;
+    uint8_t* const vs = lds + 2 * KB * D * 2;
+    auto put = [&](uint8_t* row, int ch, int off, const uint32_t (&w)[M::CH / 2]) {
+        uint8_t* p = row + (ch << 4) + off;
+        if constexpr (M::CH == 8) *(u32x4*)p = u32x4{w[0], w[1], w[2], w[3]};
+        else *(u32x2*)p = u32x2{w[0], w[1]};
+    };
+    auto store_k = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < M::NCH; ++i) {
-            const int64_t at = (row * D + (i * M::TPK + spart) * M::CH) * ESZ;
-            load_words<RW>((const uint8_t*)c.k + at, kr[i], 4);
-            load_words<RW>((const uint8_t*)c.v + at, vr[i], 4);
-        }
-        if constexpr (STORE >= RALF_KV_E4M3) {
-            kex = ((const uint8_t*)c.k_exp)[row];
-            vex = ((const uint8_t*)c.v_exp)[row];
+            uint32_t w[M::CH / 2];
+            chunk_bf16<STORE, M::CH>(kr[i], kex, w);
+            const int e = (i * M::TPK + spart) * M::CH;
+            put(ks + (buf * KB + skey) * (D * 2), (e >> 3) ^ M::kswz(skey), (e & 7) * 2, w);
         }
     };
-    auto store = [&](int blk, int buf) {
-        uint8_t* kd = lds + buf * (KB * D * 2);
-        uint8_t* vd = lds + (2 + buf) * (KB * D * 2);
-        const bool mixed = blk * KB < wg_lo || blk * KB + KB - 1 > wg_hi || bad_next;     // some row of the workgroup does not see some key of the tile
+    auto store_v = [&](int buf, int blk, uint32_t bad) {
+        const bool mixed = blk * KB < wg_lo || blk * KB + KB - 1 > wg_hi || bad;     // some row of the workgroup does not see some key of the tile
 #pragma unroll
         for (int i = 0; i < M::NCH; ++i) {
-            uint32_t kw[M::CH / 2], vw[M::CH / 2];
-            chunk_bf16<STORE, M::CH>(kr[i], kex, kw);
-            chunk_bf16<STORE, M::CH>(vr[i], vex, vw);
+            uint32_t w[M::CH / 2];
+            chunk_bf16<STORE, M::CH>(vr[i], vex, w);
             if (mixed) {
                 // values that are not there: 0.  Infinities and NaN, which 0 * inf would carry to rows that do not see them: taken out, and given to the rows that do
                 // see them when the loop is done
 #pragma unroll
                 for (int x = 0; x < M::CH / 2; ++x) {
-                    if (gone) vw[x] = 0u;
-                    else if (odd_word<RALF_KV_BF16>(vw[x])) { vw[x] = finite_word<RALF_KV_BF16>(vw[x]); s_odd = 1; }
+                    if (vgone) w[x] = 0u;
+                    else if (odd_word<RALF_KV_BF16>(w[x])) { w[x] = finite_word<RALF_KV_BF16>(w[x]); s_odd = 1; }
                 }
             }
-            const int e = (i * M::TPK + spart) * M::CH, ch = e >> 3, off = (e & 7) * 2;
-            uint8_t* kp = kd + skey * (D * 2) + ((ch ^ M::kswz(skey)) << 4) + off;
-            uint8_t* vp = vd + skey * (D * 2) + ((ch ^ M::vswz(skey)) << 4) + off;
-            if constexpr (M::CH == 8) {
-                *(u32x4*)kp = u32x4{kw[0], kw[1], kw[2], kw[3]};
-                *(u32x4*)vp = u32x4{vw[0], vw[1], vw[2], vw[3]};
-            } else {
-                *(u32x2*)kp = u32x2{kw[0], kw[1]};
-                *(u32x2*)vp = u32x2{vw[0], vw[1]};
-            }
+            const int e = (i * M::TPK + spart) * M::CH;
+            put(vs + (buf * KB + skey) * (D * 2), (e >> 3) ^ M::vswz(skey), (e & 7) * 2, w);
         }
     };
-    auto compute = [&](int blk, int buf) {
-        const uint8_t* kd = lds + buf * (KB * D * 2);
-        const uint8_t* vd = lds + (2 + buf) * (KB * D * 2);
-        const int key0 = blk * KB;
-        f32x16 st[2];
+    // scores of keys 32 kt .. of K buffer buf
+    auto scores = [&](f32x16& st, int buf, int kt) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
+        for (int i = 0; i < 16; ++i) st[i] = 0.f;
+        const int key = 32 * kt + r32;
+        const uint8_t* kp = ks + (buf * KB + key) * (D * 2);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
-            const int key = 32 * kt + r32;
-            const uint8_t* kp = kd + key * (D * 2);
+        for (int j = 0; j < D / 16; ++j) {
+            const bf16x8 kf = *(const bf16x8*)(kp + (((2 * j + h) ^ M::kswz(key)) << 4));
+            st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, q[j]), st, 0, 0, 0);
+        }
+    };
+    // what the scores are masked with and the reference follows, before their weights are taken; pb: weights taken already and not yet summed up
+    auto settle = [&](f32x16& st, int key0, uint32_t bad2, bf16x8 (&pb)[2]) {
+        if (key0 < full_lo || key0 + 31 > full_hi || bad2) {
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-                const bf16x8 kf = *(const bf16x8*)(kp + (((2 * j + h) ^ M::kswz(key)) << 4));
-                st[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, q[j]), st[kt], 0, 0, 0);
+            for (int i = 0; i < 16; ++i) {
+                const int key = key0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                const bool see = key >= lo && key <= hi && !((bad2 >> (i >> 3)) & 1u);
+                st[i] = see ? st[i] : -__builtin_inff();
             }
         }
-        if (key0 < full_lo || key0 + KB - 1 > full_hi || bad) {
+        float mx = st[0];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int o = 32 * kt + 8 * (i >> 2) + 4 * h + (i & 3);
-                    const bool see = key0 + o >= lo && key0 + o <= hi && !((bad >> (2 * kt + (i >> 3))) & 1u);
-                    st[kt][i] = see ? st[kt][i] : -__builtin_inff();
-                }
-        }
-        float mx = fmaxf(st[0][0], st[1][0]);
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[i]);
         float mo = mx;
         wave::swap32(mx, mo);
-        mx = fmaxf(m, fmaxf(mx, mo));
-        const float base = mx == -__builtin_inff() ? 0.f : mx * qs;
-        if (__any(mx > m)) {
-            const float alpha = m == -__builtin_inff() ? 0.f : exp2f_(m * qs - base);
+        mx = fmaxf(mx, mo) * qs;
+        const bool need = mx > m2 + 8.f;
+        if (__any(need)) {
+            const float mn = need ? ceilf(mx) : m2;
+            const float alpha = mn == -__builtin_inff() ? 1.f : exp2f_(m2 - mn);       // (m2 = -inf: 0; unchanged: 1)
+            m2 = mn;
             l *= alpha;
-            m = mx;
 #pragma unroll
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) acc[i][j] *= alpha;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pb[u][e] = (bf16)((float)pb[u][e] * alpha);
         }
-        float sum = 0.f;
+    };
+    auto weights = [&](const f32x16& st, bf16x8 (&pb)[2]) {
+        const float base = m2 == -__builtin_inff() ? 0.f : -m2;
+        float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                bf16x8 pb;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float p = exp2f_(fmaf(st[kt][8 * u + e], qs, -base));
-                    sum += p;
-                    pb[e] = (bf16)p;
-                }
-                const int Ls = lane & 15;
-#pragma unroll
-                for (int ct = 0; ct < D / 32; ++ct) {
-                    bf16x4 v[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int key = 32 * kt + 16 * u + 8 * x + 4 * h + (Ls >> 2), col = 32 * ct + 16 * ((lane >> 4) & 1) + (Ls & 3) * 4;
-                        v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vd + key * (D * 2) + (((col >> 3) ^ M::vswz(key)) << 4) + (col & 7) * 2));
-                    }
-                    acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7), pb, acc[ct], 0, 0, 0);
-                }
+            for (int e = 0; e < 8; ++e) {
+                const float p = exp2f_(fmaf(st[8 * u + e], qs, base));
+                if (e & 1) s1 += p;
+                else s0 += p;
+                pb[u][e] = (bf16)p;
             }
-        l += sum;               // (this half's keys only: the two are added at the end)
+        l += s0 + s1;               // (this half's keys only: the two are added at the end)
+    };
+    auto sum_up = [&](const bf16x8 (&pb)[2], int buf, int kt) {
+        const int Ls = lane & 15;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int ct = 0; ct < D / 32; ++ct) {
+                bf16x4 v[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int key = 32 * kt + 16 * u + 8 * x + 4 * h + (Ls >> 2), col = 32 * ct + 16 * ((lane >> 4) & 1) + (Ls & 3) * 4;
+                    v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vs + (buf * KB + key) * (D * 2) + (((col >> 3) ^ M::vswz(key)) << 4) + (col & 7) * 2));
+                }
+                acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7), pb[u], acc[ct], 0, 0, 0);
+            }
     };
 
-    look(sb);
-    if (sb < se) load(sb);
-    __syncthreads();            // (s_odd)
-    if (sb < se) store(sb, 0);
-    look(sb + 1);
-    __syncthreads();
-    for (int blk = sb; blk < se; ++blk) {
-        const int buf = (blk - sb) & 1;
-        bad = bad_next;
-        if (blk + 1 < se) load(blk + 1);
-        look(blk + 2);
-        if (blk * KB < wend && blk * KB + KB > wbeg) compute(blk, buf);         // (not the tiles that none of the wave's rows sees)
-        if (blk + 1 < se) store(blk + 1, buf ^ 1);
+    // The loop runs over halves of 32 keys: while the weights of one half are taken (vector unit), the scores of the next and the products of the weights before it
+    // are made (matrix unit).  Scores so run half a tile ahead and products half a tile behind: in tile j's turn K tiles j and j + 1 and V tiles j - 1 and j are in LDS,
+    // K tile j + 1 and V tile j stored there in its first half, with the one barrier behind it.
+    const int nt = se > sb ? se - sb : 0;
+    if (nt) {
+        Pages g0 = look(sb), g1 = look(sb + 1);
+        int64_t row0 = row_of(sb, g0);
+        load(c.k, c.k_exp, row0, kr, kex);
+        for (int i = threadIdx.x; i < KB * D / 8; i += 64 * M::WAVES) ((u32x4*)(vs + KB * D * 2))[i] = u32x4{0u, 0u, 0u, 0u};      // ("tile -1": values for weights of 0)
+        store_k(0);
+        load(c.v, c.v_exp, row0, vr, vex);
+        vgone = row0 < 0;
+        uint32_t bad0 = bad_of(g0), bad1 = 3u | 12u;
+        row0 = row_of(sb + 1, g1);
+        if (nt > 1) { load(c.k, c.k_exp, row0, kr, kex); bad1 = bad_of(g1); }
         __syncthreads();
+        f32x16 sa, sc;
+        bf16x8 pa[2], pc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pa[u][e] = pc[u][e] = (bf16)0.f;
+        scores(sa, 0, 0);
+        settle(sa, sb * KB, bad0 & 3u, pa);
+        for (int j = 0; j < nt; ++j) {
+            const int blk = sb + j, cur = j & 1;
+            const Pages g2 = look(blk + 2);
+            // first half: its weights; the scores of the second; the products of the tile before
+            scores(sc, cur, 1);
+            sum_up(pc, cur ^ 1, 1);
+            weights(sa, pa);
+            store_k(cur ^ 1);
+            store_v(cur, blk, bad0);
+            vgone = row0 < 0;
+            if (j + 1 < nt) load(c.v, c.v_exp, row0, vr, vex);
+            row0 = row_of(blk + 2, g2);
+            if (j + 2 < nt) load(c.k, c.k_exp, row0, kr, kex);
+            settle(sc, blk * KB + 32, bad0 >> 2, pa);
+            __syncthreads();
+            // second half: its weights; the scores of the next tile's first; the products of this tile's first
+            if (j + 1 < nt) scores(sa, cur ^ 1, 0);
+            sum_up(pa, cur, 0);
+            weights(sc, pc);
+            bad0 = bad1;
+            bad1 = bad_of(g2);
+            if (j + 1 < nt) settle(sa, (blk + 1) * KB, bad0 & 3u, pc);
+        }
+        sum_up(pc, (nt - 1) & 1, 1);
     }
+    __syncthreads();            // (s_odd)
 
     {
         if (s_odd) {            // the values taken out, to the rows that see them
@@ -794,7 +835,6 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     float lo2 = l;
     wave::swap32(l, lo2);
     l += lo2;
-    const float ml2 = m == -__builtin_inff() ? m : m * qs;
     if (a.splits > 1) {
         const int64_t at = ((int64_t)split * a.d.T + tok0 + ti) * a.d.q_heads + hq;
 #pragma unroll
@@ -802,7 +842,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 *(f32x4*)(a.part_o + at * D + 32 * ct + 8 * g + 4 * h) = f32x4{acc[ct][4 * g], acc[ct][4 * g + 1], acc[ct][4 * g + 2], acc[ct][4 * g + 3]};
-        if (h == 0) { a.part_ml[at * 2] = ml2; a.part_ml[at * 2 + 1] = l; }
+        if (h == 0) { a.part_ml[at * 2] = m2; a.part_ml[at * 2 + 1] = l; }
     } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bf16* op = (bf16*)a.d.o + (tok0 + ti) * a.d.o_ts + hq * a.d.o_hs;
