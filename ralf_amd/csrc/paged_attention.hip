@@ -510,8 +510,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
 // v_mfma_f32_32x32x16_bf16: a lane owns row (lane & 31) and of every 32 keys the sixteen 8 (i / 4) + 4 (lane / 32) + i % 4.
 //   * a tile's loads are issued a tile ahead into registers and stored to the other LDS buffer behind the products: one barrier a tile.  8-bit codes become
 //     bf16 values there, once for all waves.
-//   * LDS rows of dim elements without padding; 16-byte chunk c of a K row lies at c ^ (key & 7) -- eight lanes reading one chunk of eight keys touch all banks
-//     once -- and of a V row at c ^ 2 (key & 3), for the transposing reads (4 keys x 16 columns to 16 lanes).
+//   * LDS rows of dim elements without padding, their 16-byte chunks swizzled (kswz, vswz).
 // ------------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -524,8 +523,10 @@ struct Many {
     static constexpr int EPT = D / TPK, CH = EPT < 8 ? EPT : 8, NCH = EPT / CH;     // a thread's elements, in chunks of CH
     static constexpr int CPR = D / 8;                               // 16-byte chunks of an LDS row
     static constexpr int LDS = 2 * 2 * KB * D * 2;                  // bytes: K and V, two buffers
-    static __device__ __forceinline__ int kswz(int key) { return D >= 64 ? key & 7 : (key >> 1) & 3; }
-    static __device__ __forceinline__ int vswz(int key) { return D >= 64 ? 2 * (key & 3) : 2 * (key & 1); }
+    // where 16-byte chunk c of a row lies: c ^ kswz(key), c ^ vswz(key).  Sixteen lanes reading one chunk of sixteen keys, and 32 lanes reading 4 chunks of 4 values
+    // (the transposing read), so touch each of the 64 banks once.
+    static __device__ __forceinline__ int kswz(int key) { return D >= 128 ? key & 15 : D == 64 ? (key >> 1) & 7 : (key >> 2) & 3; }
+    static __device__ __forceinline__ int vswz(int key) { return D >= 128 ? 4 * (key & 3) : D == 64 ? 4 * ((key >> 1) & 1) : 0; }
 };
 
 // CH codes / values of a chunk, bf16 pairs
@@ -619,21 +620,20 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     const int* table = c.table + (int64_t)t.b * c.table_ld;
     const int64_t head_rows = (int64_t)c.heads * c.page;
     const int skey = threadIdx.x / M::TPK, spart = threadIdx.x % M::TPK, s4 = skey >> 4;        // the key row and part of it that this thread brings in
-    auto there = [&](int pg) { return pg >= 0 && pg < c.n_pages; };
-    typedef int Pages __attribute__((ext_vector_type(4)));       // of a tile's four sixteens: looked up one tile ahead of their loads
+    // pages of a tile's four sixteens, one to a lane (lane & 3); the keys that a wave brings in lie in one of them
+    const int lane4 = lane & 3, mine = __builtin_amdgcn_readfirstlane(s4);
     auto look = [&](int blk) {
-        auto one = [&](int s) {
-            const int k0 = blk * KB + 16 * s;
-            return blk < se && k0 < t.L ? __builtin_amdgcn_readfirstlane(table[k0 >> a.page_log2]) : -1;
-        };
-        return Pages{one(0), one(1), one(2), one(3)};
+        const int k0 = blk * KB + 16 * lane4;
+        const bool in = blk < se && k0 < t.L;
+        const int pg = table[in ? k0 >> a.page_log2 : 0];
+        return in && pg >= 0 && pg < c.n_pages ? pg : -1;
     };
-    auto bad_of = [&](const Pages g) { return (there(g[0]) ? 0u : 1u) | (there(g[1]) ? 0u : 2u) | (there(g[2]) ? 0u : 4u) | (there(g[3]) ? 0u : 8u); };
-    auto row_of = [&](int blk, const Pages g) {        // this thread's key's row of the pool (of page 0 if it is not there), negative - 1 if it is not there
-        const int pg = (s4 & 2) ? (s4 & 1) ? g[3] : g[2] : (s4 & 1) ? g[1] : g[0];
+    auto bad_of = [&](int pages) { return (uint32_t)__ballot(pages < 0) & 15u; };
+    auto row_of = [&](int blk, int pages) {             // this thread's key's row of the pool, or, if it is not there, -1 - a row of page 0
+        const int pg = __builtin_amdgcn_readlane(pages, mine);
         const int key = blk * KB + skey;
-        const int64_t row = (there(pg) ? pg : 0) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
-        return there(pg) && key < t.L ? row : -1 - row;
+        const int64_t row = (pg < 0 ? 0 : pg) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
+        return pg >= 0 && key < t.L ? row : -1 - row;
     };
     uint32_t kr[M::NCH][RW], vr[M::NCH][RW], kex = 127u, vex = 127u;
     bool vgone = false;
@@ -678,17 +678,18 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
             put(vs + (buf * KB + skey) * (D * 2), (e >> 3) ^ M::vswz(skey), (e & 7) * 2, w);
         }
     };
-    // scores of keys 32 kt .. of K buffer buf
-    auto scores = [&](f32x16& st, int buf, int kt) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.f;
-        const int key = 32 * kt + r32;
-        const uint8_t* kp = ks + (buf * KB + key) * (D * 2);
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            const bf16x8 kf = *(const bf16x8*)(kp + (((2 * j + h) ^ M::kswz(key)) << 4));
-            st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, __builtin_bit_cast(bf16x8, q[j]), st, 0, 0, 0);
-        }
+    // LDS addresses of a lane's fragments (the swizzles are exclusive ors, so a fragment's place is its number's exclusive or with the lane's own)
+    const uint32_t kaddr = r32 * (D * 2) + ((h ^ M::kswz(r32)) << 4);
+    uint32_t vaddr;
+    {
+        const int Ls = lane & 15, vkey = 4 * h + (Ls >> 2), vcol = 16 * ((lane >> 4) & 1) + (Ls & 3) * 4;
+        vaddr = 2 * KB * D * 2 + vkey * (D * 2) + (((vcol >> 3) ^ M::vswz(vkey)) << 4) + (vcol & 7) * 2;
+    }
+    auto key_frag = [&](int j, int at) { return *(const bf16x8*)(lds + (kaddr ^ (j << 5)) + at * (D * 2)); };       // at: buffer * KB + first key
+    auto value_frag = [&](int ct, int at) {
+        const uint8_t* p = lds + (vaddr ^ (ct << 6)) + at * (D * 2);
+        const bf16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, p)), v1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, p + 8 * D * 2));
+        return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     // what the scores are masked with and the reference follows, before their weights are taken; pb: weights taken already and not yet summed up
     auto settle = [&](f32x16& st, int key0, uint32_t bad2, bf16x8 (&pb)[2]) {
@@ -700,12 +701,12 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
                 st[i] = see ? st[i] : -__builtin_inff();
             }
         }
-        float mx = st[0];
+        float mx = st[0];           // (NaN is carried along: the row's weights are NaN whatever the reference)
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[i]);
+        for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, st[i]);
         float mo = mx;
         wave::swap32(mx, mo);
-        mx = fmaxf(mx, mo) * qs;
+        mx = __builtin_elementwise_maximum(mx, mo) * qs;
         const bool need = mx > m2 + 8.f;
         if (__any(need)) {
             const float mn = need ? ceilf(mx) : m2;
@@ -722,34 +723,38 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
                 for (int e = 0; e < 8; ++e) pb[u][e] = (bf16)((float)pb[u][e] * alpha);
         }
     };
-    auto weights = [&](const f32x16& st, bf16x8 (&pb)[2]) {
+    // One half's turn: the weights pb of its scores st; beside them the scores sn of the half at `knext` and the products of the weights pp with the values at `vprev`.
+    // Written in the order that it is to run in, a scheduling fence behind each step: two matrix instructions, the fragments of the step after next, two weights.
+    auto turn = [&](const f32x16& st, bf16x8 (&pb)[2], f32x16& sn, int knext, const bf16x8 (&pp)[2], int vprev) {
+        constexpr int STEPS = D / 16, EACH = 16 / STEPS > 0 ? 16 / STEPS : 1;
         const float base = m2 == -__builtin_inff() ? 0.f : -m2;
         float s0 = 0.f, s1 = 0.f;
+        bf16x8 kf[2], vf[2];
+        auto fetch = [&](int i) {
+            kf[i & 1] = key_frag(i, knext);
+            vf[i & 1] = value_frag(i % (D / 32), vprev + 16 * (i / (D / 32)));
+        };
+        fetch(0);
+        fetch(1);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int i = 0; i < 16; ++i) sn[i] = 0.f;
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float p = exp2f_(fmaf(st[8 * u + e], qs, base));
+        for (int i = 0; i < STEPS; ++i) {
+            const int u = i / (D / 32), ct = i % (D / 32);
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i & 1], __builtin_bit_cast(bf16x8, q[i]), sn, 0, 0, 0);
+            acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 1], pp[u], acc[ct], 0, 0, 0);
+            if (i + 2 < STEPS) fetch(i + 2);
+#pragma unroll
+            for (int e = i * EACH; e < (i + 1) * EACH && e < 16; ++e) {
+                const float p = exp2f_(fmaf(st[e], qs, base));
                 if (e & 1) s1 += p;
                 else s0 += p;
-                pb[u][e] = (bf16)p;
+                pb[e >> 3][e & 7] = (bf16)p;
             }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         l += s0 + s1;               // (this half's keys only: the two are added at the end)
-    };
-    auto sum_up = [&](const bf16x8 (&pb)[2], int buf, int kt) {
-        const int Ls = lane & 15;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int ct = 0; ct < D / 32; ++ct) {
-                bf16x4 v[2];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int key = 32 * kt + 16 * u + 8 * x + 4 * h + (Ls >> 2), col = 32 * ct + 16 * ((lane >> 4) & 1) + (Ls & 3) * 4;
-                    v[x] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vs + (buf * KB + key) * (D * 2) + (((col >> 3) ^ M::vswz(key)) << 4) + (col & 7) * 2));
-                }
-                acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7), pb[u], acc[ct], 0, 0, 0);
-            }
     };
 
     // The loop runs over halves of 32 keys: while the weights of one half are taken (vector unit), the scores of the next and the products of the weights before it
@@ -757,16 +762,16 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     // K tile j + 1 and V tile j stored there in its first half, with the one barrier behind it.
     const int nt = se > sb ? se - sb : 0;
     if (nt) {
-        Pages g0 = look(sb), g1 = look(sb + 1);
-        int64_t row0 = row_of(sb, g0);
-        load(c.k, c.k_exp, row0, kr, kex);
+        int pages = look(sb), pages1 = look(sb + 1);
+        int64_t row = row_of(sb, pages);
+        load(c.k, c.k_exp, row, kr, kex);
         for (int i = threadIdx.x; i < KB * D / 8; i += 64 * M::WAVES) ((u32x4*)(vs + KB * D * 2))[i] = u32x4{0u, 0u, 0u, 0u};      // ("tile -1": values for weights of 0)
         store_k(0);
-        load(c.v, c.v_exp, row0, vr, vex);
-        vgone = row0 < 0;
-        uint32_t bad0 = bad_of(g0), bad1 = 3u | 12u;
-        row0 = row_of(sb + 1, g1);
-        if (nt > 1) { load(c.k, c.k_exp, row0, kr, kex); bad1 = bad_of(g1); }
+        load(c.v, c.v_exp, row, vr, vex);
+        vgone = row < 0;
+        uint32_t bad0 = bad_of(pages), bad1 = bad_of(pages1);
+        row = row_of(sb + 1, pages1);
+        load(c.k, c.k_exp, row, kr, kex);           // (behind the last tile: a row that is not there, read from page 0 and never used)
         __syncthreads();
         f32x16 sa, sc;
         bf16x8 pa[2], pc[2];
@@ -774,32 +779,35 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) pa[u][e] = pc[u][e] = (bf16)0.f;
-        scores(sa, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sa[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_frag(i, 0), __builtin_bit_cast(bf16x8, q[i]), sa, 0, 0, 0);
         settle(sa, sb * KB, bad0 & 3u, pa);
         for (int j = 0; j < nt; ++j) {
-            const int blk = sb + j, cur = j & 1;
-            const Pages g2 = look(blk + 2);
+            const int blk = sb + j, cur = (j & 1) * KB, oth = KB - cur;
+            pages = look(blk + 2);
             // first half: its weights; the scores of the second; the products of the tile before
-            scores(sc, cur, 1);
-            sum_up(pc, cur ^ 1, 1);
-            weights(sa, pa);
-            store_k(cur ^ 1);
-            store_v(cur, blk, bad0);
-            vgone = row0 < 0;
-            if (j + 1 < nt) load(c.v, c.v_exp, row0, vr, vex);
-            row0 = row_of(blk + 2, g2);
-            if (j + 2 < nt) load(c.k, c.k_exp, row0, kr, kex);
+            turn(sa, pa, sc, cur + 32, pc, oth + 32);
+            store_k(j & 1 ^ 1);
+            store_v(j & 1, blk, bad0);
+            vgone = row < 0;
+            load(c.v, c.v_exp, row, vr, vex);
+            row = row_of(blk + 2, pages);
+            load(c.k, c.k_exp, row, kr, kex);
             settle(sc, blk * KB + 32, bad0 >> 2, pa);
             __syncthreads();
-            // second half: its weights; the scores of the next tile's first; the products of this tile's first
-            if (j + 1 < nt) scores(sa, cur ^ 1, 0);
-            sum_up(pa, cur, 0);
-            weights(sc, pc);
+            // second half: its weights; the scores of the next tile's first (of stale keys behind the last tile: not used); the products of this tile's first
+            turn(sc, pc, sa, oth, pa, cur);
             bad0 = bad1;
-            bad1 = bad_of(g2);
+            bad1 = bad_of(pages);
             if (j + 1 < nt) settle(sa, (blk + 1) * KB, bad0 & 3u, pc);
         }
-        sum_up(pc, (nt - 1) & 1, 1);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const int u = i / (D / 32), ct = i % (D / 32);
+            acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_frag(ct, ((nt - 1) & 1) * KB + 32 + 16 * u), pc[u], acc[ct], 0, 0, 0);
+        }
     }
     __syncthreads();            // (s_odd)
 
