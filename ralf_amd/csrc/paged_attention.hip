@@ -629,19 +629,18 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         return in && pg >= 0 && pg < c.n_pages ? pg : -1;
     };
     auto bad_of = [&](int pages) { return (uint32_t)__ballot(pages < 0) & 15u; };
-    auto row_of = [&](int blk, int pages) {             // this thread's key's row of the pool, or, if it is not there, -1 - a row of page 0
+    // the pool's row of the first key that this wave brings in (of page 0 if its page is not there): the same for all its lanes
+    auto row_of = [&](int blk, int pages) {
         const int pg = __builtin_amdgcn_readlane(pages, mine);
-        const int key = blk * KB + skey;
-        const int64_t row = (pg < 0 ? 0 : pg) * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
-        return pg >= 0 && key < t.L ? row : -1 - row;
+        return (pg < 0 ? 0 : pg) * head_rows + (int64_t)hk * c.page + ((blk * KB + 16 * mine) & (c.page - 1));
     };
+    const uint32_t lane_row = skey & 15, lane_at = (lane_row * D + spart * M::CH) * ESZ;
     uint32_t kr[M::NCH][RW], vr[M::NCH][RW], kex = 127u, vex = 127u;
-    bool vgone = false;
     auto load = [&](const void* base, const void* exps, int64_t row, uint32_t (&w)[M::NCH][RW], uint32_t& ex) {
-        row = row < 0 ? -1 - row : row;
+        const uint8_t* p = (const uint8_t*)base + row * (D * ESZ);
 #pragma unroll
-        for (int i = 0; i < M::NCH; ++i) load_words<RW>((const uint8_t*)base + (row * D + (i * M::TPK + spart) * M::CH) * ESZ, w[i], 4);
-        if constexpr (STORE >= RALF_KV_E4M3) ex = ((const uint8_t*)exps)[row];
+        for (int i = 0; i < M::NCH; ++i) load_words<RW>(p + lane_at + i * (M::TPK * M::CH * ESZ), w[i], 4);
+        if constexpr (STORE >= RALF_KV_E4M3) ex = ((const uint8_t*)exps + row)[lane_row];
     };
     uint8_t* const ks = lds;
     uint8_t* const vs = lds + 2 * KB * D * 2;
@@ -661,6 +660,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     };
     auto store_v = [&](int buf, int blk, uint32_t bad) {
         const bool mixed = blk * KB < wg_lo || blk * KB + KB - 1 > wg_hi || bad;     // some row of the workgroup does not see some key of the tile
+        const bool gone = ((bad >> mine) & 1u) || blk * KB + skey >= t.L;
 #pragma unroll
         for (int i = 0; i < M::NCH; ++i) {
             uint32_t w[M::CH / 2];
@@ -670,7 +670,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
                 // see them when the loop is done
 #pragma unroll
                 for (int x = 0; x < M::CH / 2; ++x) {
-                    if (vgone) w[x] = 0u;
+                    if (gone) w[x] = 0u;
                     else if (odd_word<RALF_KV_BF16>(w[x])) { w[x] = finite_word<RALF_KV_BF16>(w[x]); s_odd = 1; }
                 }
             }
@@ -726,9 +726,10 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
     // One half's turn: the weights pb of its scores st; beside them the scores sn of the half at `knext` and the products of the weights pp with the values at `vprev`.
     // Written in the order that it is to run in, a scheduling fence behind each step: two matrix instructions, the fragments of the step after next, two weights.
     auto turn = [&](const f32x16& st, bf16x8 (&pb)[2], f32x16& sn, int knext, const bf16x8 (&pp)[2], int vprev) {
-        constexpr int STEPS = D / 16, EACH = 16 / STEPS > 0 ? 16 / STEPS : 1;
+        constexpr int STEPS = D / 16;
         const float base = m2 == -__builtin_inff() ? 0.f : -m2;
         float s0 = 0.f, s1 = 0.f;
+        uint32_t w[8];
         bf16x8 kf[2], vf[2];
         auto fetch = [&](int i) {
             kf[i & 1] = key_frag(i, knext);
@@ -746,14 +747,18 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
             acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 1], pp[u], acc[ct], 0, 0, 0);
             if (i + 2 < STEPS) fetch(i + 2);
 #pragma unroll
-            for (int e = i * EACH; e < (i + 1) * EACH && e < 16; ++e) {
-                const float p = exp2f_(fmaf(st[e], qs, base));
-                if (e & 1) s1 += p;
-                else s0 += p;
-                pb[e >> 3][e & 7] = (bf16)p;
+            for (int e = STEPS > 8 ? i / 2 : i * 8 / STEPS; e < (STEPS > 8 ? i / 2 + (i & 1) : (i + 1) * 8 / STEPS); ++e) {
+                const float x = exp2f_(fmaf(st[2 * e], qs, base)), y = exp2f_(fmaf(st[2 * e + 1], qs, base));
+                s0 += x;
+                s1 += y;
+                const bf16x2 xy = {(bf16)x, (bf16)y};
+                w[e] = __builtin_bit_cast(uint32_t, xy);
+                asm volatile("" : "+v"(w[e]), "+v"(s0), "+v"(s1));         // (here, in the matrix instructions' shadow, and not where the weights are used)
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        pb[0] = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+        pb[1] = __builtin_bit_cast(bf16x8, u32x4{w[4], w[5], w[6], w[7]});
         l += s0 + s1;               // (this half's keys only: the two are added at the end)
     };
 
@@ -768,7 +773,6 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         for (int i = threadIdx.x; i < KB * D / 8; i += 64 * M::WAVES) ((u32x4*)(vs + KB * D * 2))[i] = u32x4{0u, 0u, 0u, 0u};      // ("tile -1": values for weights of 0)
         store_k(0);
         load(c.v, c.v_exp, row, vr, vex);
-        vgone = row < 0;
         uint32_t bad0 = bad_of(pages), bad1 = bad_of(pages1);
         row = row_of(sb + 1, pages1);
         load(c.k, c.k_exp, row, kr, kex);           // (behind the last tile: a row that is not there, read from page 0 and never used)
@@ -791,8 +795,7 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
             turn(sa, pa, sc, cur + 32, pc, oth + 32);
             store_k(j & 1 ^ 1);
             store_v(j & 1, blk, bad0);
-            vgone = row < 0;
-            load(c.v, c.v_exp, row, vr, vex);
+                load(c.v, c.v_exp, row, vr, vex);
             row = row_of(blk + 2, pages);
             load(c.k, c.k_exp, row, kr, kex);
             settle(sc, blk * KB + 32, bad0 >> 2, pa);
