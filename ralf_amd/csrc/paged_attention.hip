@@ -516,9 +516,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
 
-template <int D>
+template <int D, int W>
 struct Many {
-    static constexpr int WAVES = D == 256 ? 4 : 8, BM = 32 * WAVES, KB = 64;
+    static constexpr int WAVES = W, BM = 32 * WAVES, KB = 64;
     static constexpr int TPK = WAVES;                               // threads of a key row
     static constexpr int EPT = D / TPK, CH = EPT < 8 ? EPT : 8, NCH = EPT / CH;     // a thread's elements, in chunks of CH
     static constexpr int CPR = D / 8;                               // 16-byte chunks of an LDS row
@@ -559,9 +559,9 @@ __device__ __forceinline__ void chunk_bf16(const uint32_t (&raw)[STORE == RALF_K
     }
 }
 
-template <int D, int STORE>
-__global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_kernel(const Args a, int ntiles) {
-    typedef Many<D> M;
+template <int D, int STORE, int W>
+__global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const Args a, int ntiles) {
+    typedef Many<D, W> M;
     constexpr int KB = M::KB, ESZ = STORE == RALF_KV_BF16 ? 2 : 1, RW = M::CH * ESZ / 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int s_odd;
@@ -692,7 +692,13 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         return __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     // what the scores are masked with and the reference follows, before their weights are taken; pb: weights taken already and not yet summed up
-    auto settle = [&](f32x16& st, int key0, uint32_t bad2, bf16x8 (&pb)[2]) {
+    auto largest = [&](const f32x16& st) {
+        float mx = st[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, st[i]);
+        return mx;
+    };
+    auto settle = [&](f32x16& st, float mx, int key0, uint32_t bad2, bf16x8 (&pb)[2]) {
         if (key0 < full_lo || key0 + 31 > full_hi || bad2) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -700,10 +706,8 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
                 const bool see = key >= lo && key <= hi && !((bad2 >> (i >> 3)) & 1u);
                 st[i] = see ? st[i] : -__builtin_inff();
             }
+            mx = largest(st);
         }
-        float mx = st[0];           // (NaN is carried along: the row's weights are NaN whatever the reference)
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, st[i]);
         float mo = mx;
         wave::swap32(mx, mo);
         mx = __builtin_elementwise_maximum(mx, mo) * qs;
@@ -724,30 +728,31 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         }
     };
     // One half's turn: the weights pb of its scores st; beside them the scores sn of the half at `knext` and the products of the weights pp with the values at `vprev`.
-    // Written in the order that it is to run in, a scheduling fence behind each step: two matrix instructions, the fragments of the step after next, two weights.
+    // Written in the order that it is to run in, a scheduling fence behind each step: one matrix instruction, the fragment of the step after next, now and then two
+    // weights.  The scores come first, so that their largest (-> the lane's, before any mask) is known when the products are through.
     auto turn = [&](const f32x16& st, bf16x8 (&pb)[2], f32x16& sn, int knext, const bf16x8 (&pp)[2], int vprev) {
-        constexpr int STEPS = D / 16;
+        constexpr int S = D / 16, STEPS = 2 * S;
         const float base = m2 == -__builtin_inff() ? 0.f : -m2;
-        float s0 = 0.f, s1 = 0.f;
+        float s0 = 0.f, s1 = 0.f, mx = 0.f;
         uint32_t w[8];
-        bf16x8 kf[2], vf[2];
-        auto fetch = [&](int i) {
-            kf[i & 1] = key_frag(i, knext);
-            vf[i & 1] = value_frag(i % (D / 32), vprev + 16 * (i / (D / 32)));
-        };
+        bf16x8 f[3];
+        auto fetch = [&](int i) { f[i % 3] = i < S ? key_frag(i, knext) : value_frag((i - S) % (D / 32), vprev + 16 * ((i - S) / (D / 32))); };
         fetch(0);
         fetch(1);
 #pragma unroll
         for (int i = 0; i < 16; ++i) sn[i] = 0.f;
+        __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            const int u = i / (D / 32), ct = i % (D / 32);
-            sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i & 1], __builtin_bit_cast(bf16x8, q[i]), sn, 0, 0, 0);
-            acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[i & 1], pp[u], acc[ct], 0, 0, 0);
+            if (i < S) sn = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i % 3], __builtin_bit_cast(bf16x8, q[i]), sn, 0, 0, 0);
+            else {
+                const int u = (i - S) / (D / 32), ct = (i - S) % (D / 32);
+                acc[ct] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i % 3], pp[u], acc[ct], 0, 0, 0);
+            }
             if (i + 2 < STEPS) fetch(i + 2);
 #pragma unroll
-            for (int e = STEPS > 8 ? i / 2 : i * 8 / STEPS; e < (STEPS > 8 ? i / 2 + (i & 1) : (i + 1) * 8 / STEPS); ++e) {
+            for (int e = i * 8 / STEPS; e < (i + 1) * 8 / STEPS; ++e) {
                 const float x = exp2f_(fmaf(st[2 * e], qs, base)), y = exp2f_(fmaf(st[2 * e + 1], qs, base));
                 s0 += x;
                 s1 += y;
@@ -755,11 +760,17 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
                 w[e] = __builtin_bit_cast(uint32_t, xy);
                 asm volatile("" : "+v"(w[e]), "+v"(s0), "+v"(s1));         // (here, in the matrix instructions' shadow, and not where the weights are used)
             }
+            if (i == S + S / 2) {
+                mx = largest(sn);             // (NaN is carried along: the row's weights are NaN whatever the reference)
+                asm volatile("" : "+v"(mx));
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         pb[0] = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
         pb[1] = __builtin_bit_cast(bf16x8, u32x4{w[4], w[5], w[6], w[7]});
         l += s0 + s1;               // (this half's keys only: the two are added at the end)
+        return mx;
     };
 
     // The loop runs over halves of 32 keys: while the weights of one half are taken (vector unit), the scores of the next and the products of the weights before it
@@ -787,24 +798,24 @@ __global__ __launch_bounds__(64 * Many<D>::WAVES, (D == 256 ? 1 : 2)) void many_
         for (int i = 0; i < 16; ++i) sa[i] = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_frag(i, 0), __builtin_bit_cast(bf16x8, q[i]), sa, 0, 0, 0);
-        settle(sa, sb * KB, bad0 & 3u, pa);
+        settle(sa, largest(sa), sb * KB, bad0 & 3u, pa);
         for (int j = 0; j < nt; ++j) {
             const int blk = sb + j, cur = (j & 1) * KB, oth = KB - cur;
             pages = look(blk + 2);
             // first half: its weights; the scores of the second; the products of the tile before
-            turn(sa, pa, sc, cur + 32, pc, oth + 32);
+            const float mc = turn(sa, pa, sc, cur + 32, pc, oth + 32);
             store_k(j & 1 ^ 1);
             store_v(j & 1, blk, bad0);
                 load(c.v, c.v_exp, row, vr, vex);
             row = row_of(blk + 2, pages);
             load(c.k, c.k_exp, row, kr, kex);
-            settle(sc, blk * KB + 32, bad0 >> 2, pa);
+            settle(sc, mc, blk * KB + 32, bad0 >> 2, pa);
             __syncthreads();
             // second half: its weights; the scores of the next tile's first (of stale keys behind the last tile: not used); the products of this tile's first
-            turn(sc, pc, sa, oth, pa, cur);
+            const float ma = turn(sc, pc, sa, oth, pa, cur);
             bad0 = bad1;
             bad1 = bad_of(pages);
-            if (j + 1 < nt) settle(sa, (blk + 1) * KB, bad0 & 3u, pc);
+            if (j + 1 < nt) settle(sa, ma, (blk + 1) * KB, bad0 & 3u, pc);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -915,8 +926,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // many_kernel costs the same whether it holds 32 rows or 256.
 constexpr int FEW = 64;
 struct Plan {
-    int splits, few_rows, few_tiles;
-    int64_t few_grid, many_tiles;       // tiles of 16 and of 256 (128) rows; 0: the kernel is not launched
+    int splits, few_rows, few_tiles, many_waves;
+    int64_t few_grid, many_tiles;       // tiles of 16 and of 32 * many_waves rows; 0: the kernel is not launched
 };
 inline Plan plan_for(const RalfPagedAttnDesc& d) {
     Plan p = {};
@@ -938,16 +949,20 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
         s = fill < turns / 2 ? fill : turns / 2;
         s = turns < 8 ? 1 : s > even ? s : even;
     } else {
-        const int bm = d.kv.dim == 256 ? 128 : 256;
+        // 256 rows to a workgroup, one of them to a CU; 128 and two to a CU where no sequence has more (half of the waves would only wait: 64 chunks of 32 tokens on
+        // 2048, 216 -> 128 us; at 8192 rows 356 us against 333).  At dim 256 the accumulators leave room for 128 rows and one workgroup.
+        p.many_waves = d.kv.dim == 256 || most_rows <= 128 ? 4 : 8;
+        const int64_t bm = 32 * p.many_waves, slots = d.kv.dim < 256 && p.many_waves == 4 ? 512 : 256;
         p.many_tiles = rows / bm + B;
         if (B > 1) {
             p.few_rows = FEW;
             p.few_tiles = FEW / 16;
             p.few_grid = B * (FEW / 16);
         }
-        // one workgroup to a CU: cut the keys only as far as leaves every CU one, in pieces of 4 tiles at least
-        const int64_t wgs = (rows + bm - 1) / bm * heads;
-        s = 256 / wgs;
+        // cut the keys only as far as leaves every CU its workgroups, in pieces of 4 tiles at least
+        const int64_t bound = B * ((most_rows + bm - 1) / bm), other = rows / bm + (B < rows / FEW ? B : rows / FEW);
+        const int64_t wgs = (bound < other ? bound : other) * heads;
+        s = slots / (wgs > 0 ? wgs : 1);
         if (s > keys / 256) s = keys / 256;
     }
     s = s > MAX_SPLITS ? MAX_SPLITS : s;
@@ -955,6 +970,13 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     return p;
 }
 
+template <int D, int STORE, int W>
+int launch_many(const Args& a, const Plan& p, hipStream_t st) {
+    constexpr int lds = Many<D, W>::LDS;
+    if (lds >= 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(many_kernel<D, STORE, W>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    many_kernel<D, STORE, W><<<(int)(p.many_tiles * a.d.kv.heads * a.splits), 64 * W, lds, st>>>(a, (int)p.many_tiles);
+    return ralf::check_launch("paged_attention (many rows)");
+}
 template <int D, int STORE, bool F32>
 int launch(const Args& a, const Plan& p, void* stream) {
     const int64_t heads = a.d.kv.heads;
@@ -962,10 +984,7 @@ int launch(const Args& a, const Plan& p, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     if constexpr (!F32) {
         if (p.many_tiles) {
-            constexpr int lds = Many<D>::LDS;
-            if (lds >= 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(many_kernel<D, STORE>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            many_kernel<D, STORE><<<(int)(p.many_tiles * heads * a.splits), 64 * Many<D>::WAVES, lds, st>>>(a, (int)p.many_tiles);
-            const int rc = ralf::check_launch("paged_attention (many rows)");
+            const int rc = D < 256 && p.many_waves == 8 ? launch_many<D, STORE, D < 256 ? 8 : 4>(a, p, st) : launch_many<D, STORE, 4>(a, p, st);
             if (rc) return rc;
         }
     }
