@@ -4,21 +4,32 @@
 // backward pass is this kernel with `inverse`.
 //   * the angle: a position of 2^31 times a frequency of 1 has no correct bit left in 32 bits once it is taken modulo 2 pi, so the product is formed in
 //     double in TURNS (freq / 2 pi), the whole turns are dropped there and only the fraction (|f| <= 1/2) goes on in fp32 to sin / cos of pi * 2f.
-//   * one thread owns VEC pairs of one token and walks over heads: its sines and cosines are computed once and stay in registers.
+//   * one thread owns 16 bytes' worth of pairs of one token and walks over heads: its sines and cosines are computed once and stay in registers.
 //   * bound by bytes: every element is read once and written once in 16-byte pieces.
 #include "common.h"
 
 namespace {
 typedef __bf16 bf16;
-template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T v[N]; };
+// 16 bytes of elements, wherever they start: heads of an odd width put rows at any element, which the memory takes at full width
+template <typename T> struct Piece { static constexpr int N = 16 / sizeof(T); typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
 
 struct RopeArgs {
     RalfRopeDesc d;
-    int rot, pass, hg;      // chunks of VEC pairs, chunks of VEC pass-through elements, head groups
+    int rot, pass, hg;      // pieces of rotated pairs and of dims passed through, head groups
 };
 
-template <typename T, int VEC, bool ADJ>
+// a pair's turn, in fp32, rounded once
+__device__ __forceinline__ void turn(float a, float b, float c, float s, float& x, float& y) {
+    x = a * c - b * s;
+    y = b * c + a * s;
+}
+
+template <typename T, bool ADJ>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
+    constexpr int N = Piece<T>::N;
+    typedef typename Piece<T>::V V;
+    typedef T V4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T V2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
     const RalfRopeDesc& d = a.d;
     const uint32_t per = (uint32_t)(a.rot + a.pass) * a.hg;
     const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -28,16 +39,26 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     const int h0 = (int)(rem / (uint32_t)(a.rot + a.pass)), c = (int)(rem % (uint32_t)(a.rot + a.pass));
     const T* x = (const T*)d.x + t * d.x_ts;
     T* y = (T*)d.y + t * d.y_ts;
-    typedef Vec<T, VEC> V;
     if (c >= a.rot) {                                   // dims behind the rotated ones
-        const int o = d.R + (c - a.rot) * VEC;
-        for (int h = h0; h < d.H; h += a.hg) *(V*)(y + h * d.y_hs + o) = *(const V*)(x + h * d.x_hs + o);
+        const int o = d.R + (c - a.rot) * N;
+        for (int h = h0; h < d.H; h += a.hg) {
+            if (o + N <= d.D) *(V*)(y + h * d.y_hs + o) = *(const V*)(x + h * d.x_hs + o);
+            else {                                      // fewer than a piece: by halves of one
+                const T* xh = x + h * d.x_hs;
+                T* yh = y + h * d.y_hs;
+                int i = o;
+                if (d.D - i >= 4) { *(V4*)(yh + i) = *(const V4*)(xh + i); i += 4; }
+                if (d.D - i >= 2) { *(V2*)(yh + i) = *(const V2*)(xh + i); i += 2; }
+                if (d.D - i >= 1) yh[i] = xh[i];
+            }
+        }
         return;
     }
-    const int P = d.R >> 1, j0 = c * VEC;
-    float cs[VEC], sn[VEC];
+    const int P = d.R >> 1, j0 = c * N, n = P - j0 < N ? P - j0 : N;
+    float cs[N], sn[N];
 #pragma unroll
-    for (int q = 0; q < VEC; ++q) {
+    for (int q = 0; q < N; ++q) {
+        if (q >= n) { cs[q] = 1.f; sn[q] = 0.f; continue; }
         const int ax = d.axis[j0 + q];
         const bool ok = (unsigned)ax < (unsigned)d.A;
         const double turns = ok ? (double)d.pos[(int64_t)ax * d.pos_as + t] * (d.freq[j0 + q] * 0.15915494309189533577) : 0.0;
@@ -47,50 +68,61 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
         cs[q] = co;
         sn[q] = d.inverse ? -s : s;
     }
-    const int o1 = ADJ ? 2 * j0 : j0, o2 = ADJ ? 2 * j0 + VEC : P + j0;
+    const int o1 = ADJ ? 2 * j0 : j0, o2 = ADJ ? 2 * j0 + N : P + j0;
+    if (n == N) {
 #pragma unroll 2
-    for (int h = h0; h < d.H; h += a.hg) {
-        const V u = *(const V*)(x + h * d.x_hs + o1), w = *(const V*)(x + h * d.x_hs + o2);
-        V p, r;
-        if (ADJ) {
-            float e[2 * VEC];
+        for (int h = h0; h < d.H; h += a.hg) {
+            const V u = *(const V*)(x + h * d.x_hs + o1), w = *(const V*)(x + h * d.x_hs + o2);
+            V p, r;
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) { e[q] = (float)u.v[q]; e[VEC + q] = (float)w.v[q]; }
-            float o[2 * VEC];
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) {
-                o[2 * q] = e[2 * q] * cs[q] - e[2 * q + 1] * sn[q];
-                o[2 * q + 1] = e[2 * q + 1] * cs[q] + e[2 * q] * sn[q];
+            for (int q = 0; q < N; ++q) {
+                float e, f;
+                if constexpr (ADJ) {
+                    // pair q: elements 2 q, 2 q + 1 of the two pieces one behind the other
+                    turn((float)(q < N / 2 ? u[2 * q % N] : w[2 * q % N]), (float)(q < N / 2 ? u[2 * q % N + 1] : w[2 * q % N + 1]), cs[q], sn[q], e, f);
+                    if (q < N / 2) { p[2 * q % N] = (T)e; p[2 * q % N + 1] = (T)f; }
+                    else { r[2 * q % N] = (T)e; r[2 * q % N + 1] = (T)f; }
+                } else {
+                    turn((float)u[q], (float)w[q], cs[q], sn[q], e, f);
+                    p[q] = (T)e;
+                    r[q] = (T)f;
+                }
             }
+            *(V*)(y + h * d.y_hs + o1) = p;
+            *(V*)(y + h * d.y_hs + o2) = r;
+        }
+    } else {                                            // the last pairs of a number that is no multiple of a piece
+        for (int h = h0; h < d.H; h += a.hg) {
+            const T* xh = x + h * d.x_hs;
+            T* yh = y + h * d.y_hs;
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) { p.v[q] = (T)o[q]; r.v[q] = (T)o[VEC + q]; }
-        } else {
-#pragma unroll
-            for (int q = 0; q < VEC; ++q) {
-                const float m = (float)u.v[q], n = (float)w.v[q];
-                p.v[q] = (T)(m * cs[q] - n * sn[q]);
-                r.v[q] = (T)(n * cs[q] + m * sn[q]);
+            for (int q = 0; q < N; ++q) {
+                if (q >= n) continue;
+                const int i1 = ADJ ? 2 * (j0 + q) : j0 + q, i2 = ADJ ? i1 + 1 : P + j0 + q;
+                float e, f;
+                turn((float)xh[i1], (float)xh[i2], cs[q], sn[q], e, f);
+                yh[i1] = (T)e;
+                yh[i2] = (T)f;
             }
         }
-        *(V*)(y + h * d.y_hs + o1) = p;
-        *(V*)(y + h * d.y_hs + o2) = r;
     }
 }
 
-template <typename T, int VEC>
+template <typename T>
 int launch(const RalfRopeDesc& d, void* stream) {
     RopeArgs a;
     a.d = d;
-    a.rot = d.R / 2 / VEC;
-    a.pass = d.x == d.y ? 0 : (d.D - d.R) / VEC;
+    const int n = Piece<T>::N;
+    a.rot = (d.R / 2 + n - 1) / n;
+    a.pass = d.x == d.y ? 0 : (d.D - d.R + n - 1) / n;
     // one head group = the angles once per token; more of them only as far as the launch would otherwise leave the card's 256 CUs short of threads
     const int64_t per = (int64_t)(a.rot + a.pass) * d.T;
     const int64_t want = ((int64_t)1 << 18) / per;
     a.hg = (int)(want < 1 ? 1 : want > d.H ? d.H : want);
     const int64_t blocks = (per * a.hg + 255) / 256;
     RALF_REQUIRE(blocks < ((int64_t)1 << 31) && (int64_t)(a.rot + a.pass) * a.hg < ((int64_t)1 << 31), "rope_axes: too many elements for one launch");
-    if (d.adjacent) rope_kernel<T, VEC, true><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
-    else rope_kernel<T, VEC, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
+    if (d.adjacent) rope_kernel<T, true><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
+    else rope_kernel<T, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
     return ralf::check_launch("rope_axes");
 }
 }  // namespace
@@ -106,17 +138,5 @@ extern "C" int ralf_rope_axes(const RalfRopeDesc* dp, void* stream) {
     RALF_REQUIRE(d.x && d.y && d.pos && d.freq && d.axis, "rope_axes: null pointer");
     RALF_REQUIRE((d.T == 1 || d.y_ts > 0) && (d.H == 1 || d.y_hs > 0), "rope_axes: the output's rows overlap");
     RALF_REQUIRE(d.x != d.y || (d.x_ts == d.y_ts && d.x_hs == d.y_hs), "rope_axes: in place needs one set of strides");
-    const int P = d.R / 2, el = d.dtype == RALF_BF16 ? 2 : 4;
-    auto fits = [&](int vec) {     // every piece a whole, aligned vector
-        const uintptr_t by = (uintptr_t)vec * el;
-        return P % vec == 0 && (d.D - d.R) % vec == 0 && d.x_ts % vec == 0 && d.x_hs % vec == 0 && d.y_ts % vec == 0 && d.y_hs % vec == 0 &&
-               (uintptr_t)d.x % by == 0 && (uintptr_t)d.y % by == 0;
-    };
-    if (d.dtype == RALF_BF16) {
-        if (fits(8)) return launch<bf16, 8>(d, stream);
-        if (fits(4)) return launch<bf16, 4>(d, stream);
-        return launch<bf16, 1>(d, stream);
-    }
-    if (fits(4)) return launch<float, 4>(d, stream);
-    return launch<float, 1>(d, stream);
+    return d.dtype == RALF_BF16 ? launch<bf16>(d, stream) : launch<float>(d, stream);
 }

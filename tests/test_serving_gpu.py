@@ -26,7 +26,7 @@ def bits(t):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("T,H,D,sections,adjacent,far", [
     (1, 1, 2, (1,), False, 3), (1, 16, 32, (16,), False, 50), (5, 3, 80, (16, 16), True, 1000), (33, 2, 128, (16, 24, 24), False, 2 ** 31 - 40), (33, 2, 128, (16, 24, 24), True, 2 ** 20),
-    (7, 5, 66, (33,), False, 7), (7, 5, 66, (30, 3), True, 7), (700, 1, 64, (3, 5, 4, 20), False, 100), (9, 40, 256, (64, 64), False, -2 ** 31 + 40), (257, 3, 98, (33,), False, 11)])
+    (7, 5, 66, (33,), False, 7), (7, 5, 66, (30, 3), True, 7), (700, 1, 64, (3, 5, 4, 20), False, 100), (9, 40, 256, (64, 64), False, -2 ** 31 + 40), (257, 3, 98, (33,), False, 11), (6, 2, 71, (33,), True, 3), (6, 2, 135, (64,), False, 3)])
 def test_rope(dtype, T, H, D, sections, adjacent, far):
     from ralf_amd import ops
 
