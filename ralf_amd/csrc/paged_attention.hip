@@ -943,9 +943,9 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
         const int64_t tiles = d.T * ((G + 15) / 16), wgs = (p.few_grid < tiles ? p.few_grid : tiles) * heads;
         // Splits of the keys.  A wave takes `turns` blocks of 32 keys one behind the other; two workgroups to a CU run at once.  Splitting costs the join (5 us, some 6
         // turns), so short axes stay whole; longer ones are cut until the card is full or a wave has two turns left, and to 16 turns at most, so that sequences of
-        // different lengths even out (64 sequences of 2048 - 8192: 154 us against 162 in one piece).
+        // different lengths even out (64 sequences of 2048 - 8192: 154 us against 162 in one piece) -- but no further than 4096 workgroups, which even out by themselves.
         const int64_t turns = (keys + 127) / 128;
-        const int64_t fill = (512 + wgs - 1) / wgs, even = (turns + 15) / 16;
+        const int64_t fill = (512 + wgs - 1) / wgs, enough = (4096 + wgs - 1) / wgs, even = (turns + 15) / 16 < enough ? (turns + 15) / 16 : enough;
         s = fill < turns / 2 ? fill : turns / 2;
         s = turns < 8 ? 1 : s > even ? s : even;
     } else {

@@ -1015,18 +1015,18 @@ class ScalePEDropFn(Function):
 
 
 class RopeAxesFn(Function):
-    """rotary positions with several axes; the gradient is the rotation by the opposite angles"""
+    """rotary positions with several axes; the gradient is the rotation by the opposite angles (and so is the gradient's gradient)"""
 
     @staticmethod
-    def forward(ctx, x, pos, freq, axis, adjacent):
+    def forward(ctx, x, pos, freq, axis, adjacent, inverse):
         ctx.save_for_backward(pos, freq, axis)
-        ctx.adjacent = adjacent
-        return ops.rope_axes(x, pos, freq, axis, adjacent=adjacent)
+        ctx.cfg = (adjacent, inverse)
+        return ops.rope_axes(x, pos, freq, axis, adjacent=adjacent, inverse=inverse)
 
     @staticmethod
     def backward(ctx, dy):
-        pos, freq, axis = ctx.saved_tensors
-        return ops.rope_axes(dy if dy.stride(-1) == 1 else dy.contiguous(), pos, freq, axis, adjacent=ctx.adjacent, inverse=True), None, None, None, None
+        adjacent, inverse = ctx.cfg
+        return RopeAxesFn.apply(dy if dy.stride(-1) == 1 else dy.contiguous(), *ctx.saved_tensors, adjacent, not inverse), None, None, None, None, None
 
 
 def _capturing():
@@ -1039,7 +1039,7 @@ def rope_axes(x, pos, freq, axis, adjacent=False):
     The gradient of a rotation is ops.rope_axes(dy, ..., inverse=True), which can be captured."""
     if x.requires_grad and x.is_leaf and torch.is_grad_enabled() and _capturing():
         raise RuntimeError("rope_axes: the gradient of a leaf inside a graph capture; use ops.rope_axes(dy, ..., inverse=True) there, or pass the leaf without requires_grad")
-    return RopeAxesFn.apply(x, pos, freq, axis, adjacent)
+    return RopeAxesFn.apply(x, pos, freq, axis, adjacent, False)
 
 
 class EmbedFn(Function):

@@ -92,6 +92,18 @@ def test_rope_gradient(dtype, adjacent):
         assert not g[:, 1:].any()
 
 
+def test_rope_gradient_of_the_gradient():
+    from ralf_amd import functional
+
+    freq, axis = torch.full((4,), 0.3, dtype=torch.float64).cuda(), torch.zeros(4, dtype=torch.int32).cuda()
+    pos = torch.arange(5).view(1, 5).cuda()
+    x, dy = rnd(5, 2, 8, seed=1).cuda().requires_grad_(True), rnd(5, 2, 8, seed=2).cuda().requires_grad_(True)
+    g, = torch.autograd.grad(functional.rope_axes(x, pos, freq, axis), x, dy, create_graph=True)
+    gg, = torch.autograd.grad(g, dy, rnd(5, 2, 8, seed=3).cuda())
+    want, e = O.rope(rnd(5, 2, 8, seed=3), pos.cpu(), freq.cpu(), axis.cpu(), False)
+    O.check(gg, want, e + O.U32 * want.abs(), "second gradient")
+
+
 # ---------------------------------------------------------------------------------------------- the cache
 def make(lens, new, heads, dim, page, store, dtype, seed, spare=2, garbage=True):
     """a pool whose unwritten cells hold what must not be looked at, page tables in random order, sequences filled with values"""
@@ -328,6 +340,36 @@ def test_attention_bad_pages(store):
     out = ops.paged_attention(q.cuda(), pool, table.cuda(), q_start.cuda(), kv_len.cuda())
     want, e, _ = O.attention(q, *O.pool_values(pool), table, q_start, kv_len, 0.125, p_step=O.half_step(BF16))
     O.check(out, want, e + O.half_step(BF16) * (want.abs() + e), "bad pages")
+
+
+@pytest.mark.parametrize("B", [65, 200, 4300])
+@pytest.mark.parametrize("new", [0, 1, 40])
+def test_many_sequences(B, new):
+    """more sequences than a wave has lanes, and than its squares: new = 0: one or no new token each, otherwise one of them brings a chunk; page table rows of a wider pitch"""
+    from ralf_amd import ops
+
+    lens = [1 + b % 5 for b in range(B)]
+    fresh = [min(t, (b * 7 % 3 > 0) * 1) for b, t in enumerate(lens)]
+    if new:
+        lens[B // 2], fresh[B // 2] = 70, new
+    pool, table, q_start, kv_len = make(lens, fresh, 1, 32, 16, BF16, BF16, seed=B)
+    wide = torch.full((B, table.shape[1] + 3), 2 ** 30, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table.cuda()
+    strided = wide[:, :table.shape[1]]
+    T = int(q_start[-1])
+    q, k, v = rnd(T, 2, 32, seed=1, dtype=BF16), rnd(T, 1, 32, seed=2, dtype=BF16), rnd(T, 1, 32, seed=3, dtype=BF16)
+    ops.paged_kv_write(pool, k.cuda(), v.cuda(), strided, q_start.cuda(), kv_len.cuda())
+    start = torch.tensor([0] + lens).cumsum(0).int()
+    rk, _ = ops.paged_kv_read(pool, strided, kv_len.cuda(), start.cuda(), int(start[-1]))
+    held = O.pool_values(pool)
+    rows = torch.tensor([(b, p) for b, t in enumerate(lens) for p in range(t)])
+    assert torch.equal(rk.cpu().double(), held[0][table[rows[:, 0], rows[:, 1] // 16].long(), :, rows[:, 1] % 16])
+    newest = torch.tensor([int(start[b]) + t - n + i for b, (t, n) in enumerate(zip(lens, fresh)) for i in range(n)])
+    assert torch.equal(rk.cpu()[newest], k)
+    for kw in (dict(), dict(max_q=max(fresh), max_kv=max(lens))):
+        out = ops.paged_attention(q.cuda(), pool, strided, q_start.cuda(), kv_len.cuda(), **kw)
+        want, e, _ = O.attention(q, *held, table, q_start, kv_len, 32 ** -0.5, p_step=O.half_step(BF16))
+        O.check(out, want, e + O.half_step(BF16) * (want.abs() + e), "many sequences")
 
 
 def test_attention_longer_than_the_table():
