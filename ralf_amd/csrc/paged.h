@@ -27,6 +27,26 @@ __device__ __forceinline__ int count_le(F key, int n, int64_t at, int lane) {
     return base + __popcll(__ballot(below));
 }
 
+// The sequence b of row t (ends: start + 1, so that rows ends[b - 1] .. ends[b] - 1 are b's; b = B behind the last), ends[b] and kv_len[b], the same in all lanes.
+// Up to 64 sequences: one lane to each, everything in one trip to memory.
+struct Owner { int b, end, len; };
+__device__ __forceinline__ Owner owner_of(const int* ends, const int* kv_len, int B, int64_t t, int lane) {
+    Owner o;
+    if (B <= 64) {
+        const int i = lane < B ? lane : B - 1, e = ends[i], n = kv_len[i];
+        o.b = __popcll(__ballot(lane < B && e <= t));
+        const int at = o.b < B ? o.b : B - 1;
+        o.end = __builtin_amdgcn_readlane(e, at);
+        o.len = __builtin_amdgcn_readlane(n, at);
+    } else {
+        o.b = count_le([&](int i) { return (int64_t)ends[i]; }, B, t, lane);
+        const int at = o.b < B ? o.b : B - 1;
+        o.end = ends[at];
+        o.len = kv_len[at];
+    }
+    return o;
+}
+
 // the exponent byte of a row whose largest magnitude has the bits u: 127 + e, e the smallest integer with max <= LARGEST * 2^e and at least -100;
 // 255 if the row holds an infinity or a NaN (their bits are the largest)
 template <int STORE>

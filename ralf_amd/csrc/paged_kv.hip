@@ -93,9 +93,9 @@ __global__ __launch_bounds__(256) void write_kernel(const WriteArgs a) {
     const int lane = threadIdx.x & 63, e0 = (lane % LANES) * 8;
     const int64_t nw = (int64_t)gridDim.x * 4;
     for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < a.T; t += nw) {
-        const int b = count_le([&](int i) { return (int64_t)a.q_start[i + 1]; }, c.B, t, lane);
-        if (b >= c.B) continue;
-        const int64_t cell = place(c, b, (int64_t)c.kv_len[b] - a.q_start[b + 1] + t);
+        const Owner w = owner_of(a.q_start + 1, c.kv_len, c.B, t, lane);
+        if (w.b >= c.B) continue;
+        const int64_t cell = place(c, w.b, (int64_t)w.len - w.end + t);
         if (cell < 0) continue;
         // (a whole row is in or out: the exchange of its largest magnitude stays within rows.  Several rows' loads in flight at once -- 2 or 4 -- measured slower,
         //  22-24 against 17 us at 10 600 tokens of 2 x 8 x 128: the registers cost more waves than the loads gained)
@@ -118,10 +118,10 @@ __global__ __launch_bounds__(256) void read_kernel(const ReadArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t nw = (int64_t)gridDim.x * 4;
     for (int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); n < a.rows; n += nw) {
-        const int b = count_le([&](int i) { return (int64_t)a.start[i + 1]; }, c.B, n, lane);
-        if (b >= c.B) continue;
-        const int64_t p = n - a.start[b];
-        const int64_t cell = p < c.kv_len[b] ? place(c, b, p) : -1;
+        const Owner w = owner_of(a.start + 1, c.kv_len, c.B, n, lane);
+        if (w.b >= c.B) continue;
+        const int64_t p = n - a.start[w.b];
+        const int64_t cell = p < w.len ? place(c, w.b, p) : -1;
         const int e0 = (lane % LANES) * 8;
 #pragma unroll 2
         for (int r = lane / LANES; r < 2 * c.heads; r += RI) {
