@@ -512,6 +512,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
 //     bf16 values there, once for all waves.
 //   * LDS rows of dim elements without padding, their 16-byte chunks swizzled (kswz, vswz).
 // ------------------------------------------------------------------------------------------------
+template <int N> struct Const { static constexpr int value = N; };
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
         for (int i = 1; i < 16; ++i) mx = __builtin_elementwise_maximum(mx, st[i]);
         return mx;
     };
-    auto settle = [&](f32x16& st, float mx, int key0, uint32_t bad2, bf16x8 (&pb)[2]) {
+    auto settle = [&](f32x16& st, float mx, int key0, uint32_t bad2, bf16x8 (&pb)[2]) __attribute__((always_inline)) {
         if (key0 < full_lo || key0 + 31 > full_hi || bad2) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -730,7 +731,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     // One half's turn: the weights pb of its scores st; beside them the scores sn of the half at `knext` and the products of the weights pp with the values at `vprev`.
     // Written in the order that it is to run in, a scheduling fence behind each step: one matrix instruction, the fragment of the step after next, now and then two
     // weights.  The scores come first, so that their largest (-> the lane's, before any mask) is known when the products are through.
-    auto turn = [&](const f32x16& st, bf16x8 (&pb)[2], f32x16& sn, int knext, const bf16x8 (&pp)[2], int vprev) {
+    auto turn = [&](const f32x16& st, bf16x8 (&pb)[2], f32x16& sn, int knext, const bf16x8 (&pp)[2], int vprev) __attribute__((always_inline)) {
         constexpr int S = D / 16, STEPS = 2 * S;
         const float base = m2 == -__builtin_inff() ? 0.f : -m2;
         float s0 = 0.f, s1 = 0.f, mx = 0.f;
@@ -799,14 +800,16 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key_frag(i, 0), __builtin_bit_cast(bf16x8, q[i]), sa, 0, 0, 0);
         settle(sa, largest(sa), sb * KB, bad0 & 3u, pa);
-        for (int j = 0; j < nt; ++j) {
-            const int blk = sb + j, cur = (j & 1) * KB, oth = KB - cur;
+        // (one tile with buffer 0 and one with buffer 1 current, so that LDS addresses are constants apart: 24 vector additions a tile less)
+        auto tile = [&](auto which, int j) __attribute__((always_inline)) {
+            const int BUF = which.value, cur = BUF * KB, oth = KB - cur;
+            const int blk = sb + j;
             pages = look(blk + 2);
             // first half: its weights; the scores of the second; the products of the tile before
             const float mc = turn(sa, pa, sc, cur + 32, pc, oth + 32);
-            store_k(j & 1 ^ 1);
-            store_v(j & 1, blk, bad0);
-                load(c.v, c.v_exp, row, vr, vex);
+            store_k(BUF ^ 1);
+            store_v(BUF, blk, bad0);
+            load(c.v, c.v_exp, row, vr, vex);
             row = row_of(blk + 2, pages);
             load(c.k, c.k_exp, row, kr, kex);
             settle(sc, mc, blk * KB + 32, bad0 >> 2, pa);
@@ -816,6 +819,15 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
             bad0 = bad1;
             bad1 = bad_of(pages);
             if (j + 1 < nt) settle(sa, ma, (blk + 1) * KB, bad0 & 3u, pc);
+        };
+        if constexpr (D < 256) {
+            for (int j = 0; j < nt; j += 2) {
+                tile(Const<0>{}, j);
+                if (j + 1 < nt) tile(Const<1>{}, j + 1);
+            }
+        } else {                // (no registers for two copies)
+            struct Which { int value; };
+            for (int j = 0; j < nt; ++j) tile(Which{j & 1}, j);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {

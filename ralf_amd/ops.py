@@ -1134,10 +1134,15 @@ def _one_device(what, first, *others):
 
 
 def _rows3(t, what):
-    """[T, heads, dim] with a contiguous last dim -> its strides in elements"""
+    """[T, heads, dim] with a contiguous last dim -> (token stride, head stride) in elements; a dim of size 1 has a stride of 0, whatever the tensor says"""
     st = t.stride()
     assert len(st) == 3 and (st[2] == 1 or t.shape[2] == 1), f"{what}: [tokens, heads, dim] with a contiguous last dim, got {tuple(t.shape)} with strides {st}"
-    return st
+    return st[0] if t.shape[0] > 1 else 0, st[1] if t.shape[1] > 1 else 0
+
+
+def _empty_as(t):
+    """a contiguous tensor of t's shape and type"""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _ptr(t):
@@ -1175,7 +1180,7 @@ def rope_axes(x, pos, freq, axis, *, adjacent=False, inverse=False, out=None):
     P = freq.shape[0]
     assert 0 < 2 * P <= D, f"rope_axes: {P} pairs in a head of {D}"
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+        out = _empty_as(x)
         ys = (H * D, D)
     else:
         assert out.shape == x.shape and out.dtype is x.dtype, "rope_axes: out has x's shape and type"
@@ -1236,7 +1241,7 @@ def _starts(t, B, what):
 
 def paged_kv_write(pool, k, v, table, q_start, kv_len):
     """the newest tokens of every sequence into the cache, quantised on the way where it holds 8 bits (ralf_paged_kv_write): k, v [T, heads, dim] (any token / head
-    strides of multiples of 8), rows q_start[b] .. q_start[b + 1] - 1 = positions kv_len[b] - n .. kv_len[b] - 1.  kv_len counts them already.  table int32
+    strides of multiples of 8, 16-byte aligned), rows q_start[b] .. q_start[b + 1] - 1 = positions kv_len[b] - n .. kv_len[b] - 1.  kv_len counts them already.  table int32
     [B, pages per sequence]: a page being written belongs to one sequence.  Rows behind q_start[B] are not stored."""
     d, held = _paged("paged_kv_write", pool, table, kv_len)
     _starts(q_start, d.B, "paged_kv_write: q_start")
@@ -1273,7 +1278,7 @@ _I32_MAX = 2 ** 31 - 1
 
 def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True, window=0, max_q=None, max_kv=None, out=None):
     """attention of every sequence's newest tokens over its pages (ralf_paged_attention) -> [T, q_heads, dim]: q [T, q_heads, dim], rows as in paged_kv_write (call it
-    first: a token sees its own key); q_heads a multiple of the cache's heads.  causal: position p sees keys <= p; window > 0: only the last `window` of them.
+    first: a token sees its own key), q_heads a multiple of the cache's heads; any token / head strides of multiples of 8, 16-byte aligned, here and in out.  causal: position p sees keys <= p; window > 0: only the last `window` of them.
     q bf16 reads caches of bf16 and 8 bits, q fp32 those of fp32 and 8 bits.  A row without a key gives zeros.  max_q / max_kv: the host's upper bounds of the
     new tokens and of kv_len of one sequence; they steer how the work is split (a captured graph keeps its split), not what is computed.
     Rows behind q_start[B] are not written."""
@@ -1288,7 +1293,7 @@ def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True,
     max_q, max_kv = max_q or 0, max_kv or 0
     assert window >= 0 and max_q >= 0 and max_kv >= 0, "paged_attention: negative window or bound"
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        out = _empty_as(q)
         os_ = (Hq * D, D)
     else:
         assert out.shape == q.shape and out.dtype is q.dtype, "paged_attention: out has q's shape and type"
@@ -1343,7 +1348,7 @@ def logits_process(logits, tokens=None, lens=None, *, prompt_lens=None, repetiti
     else:
         assert mask_row is None, "logits_process: mask_row without masks"
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=logits.device)
+        out = _empty_as(logits)
         ld_out = V
     else:
         os_ = out.stride()

@@ -303,18 +303,18 @@ def test_attention_bounds_only_steer(wrong):
     run_attention([300, 200], [150, 3], 4, 2, 64, 16, BF16, BF16, seed=8, **wrong)
 
 
-@pytest.mark.parametrize("n", [1, 6, 70, 300])
-@pytest.mark.parametrize("store,dtype", [(F32, F32), (BF16, BF16), (E4M3, BF16)])
-def test_attention_hidden_values_stay_hidden(store, dtype, n):
+@pytest.mark.parametrize("n,past", [(1, 37), (6, 37), (70, 37), (300, 37), (3, 6000), (100, 6000)])
+@pytest.mark.parametrize("store,dtype", [(F32, F32), (BF16, BF16), (E4M3, BF16), (E4M3, F32), (I8, BF16), (I8, F32)])
+def test_attention_hidden_values_stay_hidden(store, dtype, n, past):
     """infinities and NaN in keys and values of tokens that a row does not see leave it alone; the rows that see them get them"""
     def change(q, k, v, pool, table):
         v[n // 2, 0, 3], v[n // 2, 1, 4], v[n - 1, 0, 5], v[n - 1, 0, 6] = math.nan, math.inf, -math.inf, math.nan
         k[n - 1, 1, 0] = math.nan
 
-    out, want = run_attention([n + 37], [n], 4, 2, 64, 16, store, dtype, seed=6, change=change)
+    out, want = run_attention([n + past], [n], 4, 2, 64, 16, store, dtype, seed=6, change=change)
     if n > 6:
         assert torch.isfinite(out[:n // 2]).all() and not torch.isfinite(out).all()
-    run_attention([n + 37], [n], 4, 2, 64, 16, store, dtype, seed=6, change=change, window=5)
+    run_attention([n + past], [n], 4, 2, 64, 16, store, dtype, seed=6, change=change, window=5)
 
 
 def test_attention_infinite_scores():
@@ -340,6 +340,38 @@ def test_attention_bad_pages(store):
     out = ops.paged_attention(q.cuda(), pool, table.cuda(), q_start.cuda(), kv_len.cuda())
     want, e, _ = O.attention(q, *O.pool_values(pool), table, q_start, kv_len, 0.125, p_step=O.half_step(BF16))
     O.check(out, want, e + O.half_step(BF16) * (want.abs() + e), "bad pages")
+
+
+@pytest.mark.parametrize("store,dtype", [(BF16, BF16), (I8, F32)])
+def test_empty_pool(store, dtype):
+    """a cache without a page: nothing stored, zeros read, zeros attended"""
+    from ralf_amd import ops
+
+    pool = ops.paged_kv_pool(0, 16, 2, 32, store)
+    table, one = torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.tensor([5], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    k = rnd(3, 2, 32, dtype=dtype).cuda()
+    ops.paged_kv_write(pool, k, k, table, start, one)
+    assert not ops.paged_kv_read(pool, table, one, start, 3)[0].any()
+    assert not ops.paged_attention(k, pool, table, start, one).any()
+
+
+def test_strides_of_single_tokens_and_heads():
+    """a dim of size 1 may have any stride"""
+    from ralf_amd import ops
+
+    pool, table, q_start, kv_len = make([20], [1], 1, 64, 16, BF16, BF16, seed=2)
+    q = rnd(1, 3, 64, seed=3, dtype=BF16).cuda()
+    k = rnd(1, 1, 64, seed=4, dtype=BF16).cuda()
+    freq, axis = ops.rope_table((32,), device="cuda")
+    pos = torch.tensor([[7]]).cuda()
+    odd = lambda t: t.as_strided(t.shape, (193 if t.shape[0] == 1 else t.stride(0), 77 if t.shape[1] == 1 else t.stride(1), 1))    # noqa: E731
+    assert torch.equal(ops.rope_axes(odd(q), pos, freq, axis), ops.rope_axes(q, pos, freq, axis))
+    ops.paged_kv_write(pool, odd(k), odd(k), table.cuda(), q_start.cuda(), kv_len.cuda())
+    pg, r = cells(table, 0, 19, 16)
+    assert torch.equal(pool.k[pg, 0, r], k[0, 0])
+    args = (pool, table.cuda(), q_start.cuda(), kv_len.cuda())
+    assert torch.equal(ops.paged_attention(odd(q), *args, out=odd(torch.empty_like(q))), ops.paged_attention(q, *args))
 
 
 @pytest.mark.parametrize("B", [65, 200, 4300])
