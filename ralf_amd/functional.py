@@ -1026,7 +1026,10 @@ class RopeAxesFn(Function):
     @staticmethod
     def backward(ctx, dy):
         adjacent, inverse = ctx.cfg
-        return RopeAxesFn.apply(dy if dy.stride(-1) == 1 else dy.contiguous(), *ctx.saved_tensors, adjacent, not inverse), None, None, None, None, None
+        dy = dy if dy.stride(-1) == 1 else dy.contiguous()
+        if torch.is_grad_enabled():         # (create_graph)
+            return RopeAxesFn.apply(dy, *ctx.saved_tensors, adjacent, not inverse), None, None, None, None, None
+        return ops.rope_axes(dy, *ctx.saved_tensors, adjacent=adjacent, inverse=not inverse), None, None, None, None, None
 
 
 def _capturing():
