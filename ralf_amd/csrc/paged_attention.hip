@@ -11,8 +11,9 @@
 //   fp32: v_mfma_f32_16x16x4_f32 on an fp32 cache; on 8-bit codes three bf16 products, the query and the probabilities in three bf16 parts (split3).
 // Running maximum and sum of the softmax in fp32; exponentials base 2 with log2(e) folded into the scale.
 //
-// Masks.  A row that has seen no key keeps max = -inf, sum = 0 and gives zeros.  Keys behind kv_len and keys on bad pages are zeroed as they are loaded; a later
-// token's or an out-of-window value that is an infinity or a NaN must not reach a row through 0 * inf: see below.
+// Masks.  A row that has seen no key keeps max = -inf, sum = 0 and gives zeros.  Values behind kv_len and on bad pages count as zeros; a later
+// token's or an out-of-window value that is an infinity or a NaN must not reach a row through 0 * inf: such values are taken out of the products of partly visible
+// blocks and added, behind the loop, to the rows that see them.
 #include "paged.h"
 
 namespace {
@@ -78,8 +79,10 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int w, int lane, int pe
 }
 
 // ------------------------------------------------------------------------------------------------
-// few rows: 16 to a workgroup, its 4 waves take blocks of 32 keys in turn (a long axis and few rows: the keys are what there is to divide).
-// K and V go from memory straight into registers, each byte once per 16 rows.
+// few rows: 16 to a workgroup, its 4 waves take blocks of 32 or 64 keys in turn (a long axis and few rows: the keys are what there is to divide).
+// K and V go from memory straight into registers, each byte once per 16 rows; a block's loads are issued a block ahead of its products and its pages looked up
+// two ahead, which keeps 60 - 130 KB in flight to a CU.  Bound by bytes: 64 sequences of 2048 - 8192 tokens, 8 key heads of 128: e4m3 684 MB in 153 us (4.5 TB/s; without
+// the loads ahead 450 us), bf16 4.8 TB/s; a copy reaches 4.9 on this card.
 // ------------------------------------------------------------------------------------------------
 // The shapes of a lane's share of a block of NT sixteens of keys.  Of a key row it holds EPL consecutive elements (16 bytes) of every 4 EPL -- the contraction over
 // dims may run in any order, as long as the query's registers follow the same one -- and of four value rows of each sixteen CPL columns.
@@ -506,11 +509,16 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------
-// many rows: 32 to a wave, 8 waves (4 at dim 256) share tiles of 64 keys in LDS, each byte from memory once per 256 (128) rows.
+// many rows: 32 to a wave, 8 (4) waves share tiles of 64 keys in LDS, each byte from memory once per 256 (128) rows.
 // v_mfma_f32_32x32x16_bf16: a lane owns row (lane & 31) and of every 32 keys the sixteen 8 (i / 4) + 4 (lane / 32) + i % 4.
 //   * a tile's loads are issued a tile ahead into registers and stored to the other LDS buffer behind the products: one barrier a tile.  8-bit codes become
 //     bf16 values there, once for all waves.
 //   * LDS rows of dim elements without padding, their 16-byte chunks swizzled (kswz, vswz).
+//   * scores run half a tile ahead of their weights and products half a tile behind, step by step in one stream of instructions: the vector unit's 16 exponentials a
+//     lane and half (as long as 8 matrix instructions) run in the matrix unit's shadow.
+// 2048 new on 8192 cached tokens, 32 / 8 heads of 128: 316 us, 980 TFLOP/s (a large plain product: 1611), both units half busy at a clock of 2.0 GHz.  Left out one at a
+// time: staging - 46 us, weights - 43, settling - 11; bare matrix instructions, LDS reads and barriers 229 us.  Loads straight into LDS (6 us slower), fragments 4 or 6
+// steps ahead, two workgroups of 4 waves to a CU (+ 23) and other wave priorities gained nothing.
 // ------------------------------------------------------------------------------------------------
 template <int N> struct Const { static constexpr int value = N; };
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -962,7 +970,7 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
         s = turns < 8 ? 1 : s > even ? s : even;
     } else {
         // 256 rows to a workgroup, one of them to a CU; 128 and two to a CU where no sequence has more (half of the waves would only wait: 64 chunks of 32 tokens on
-        // 2048, 216 -> 128 us; at 8192 rows 356 us against 333).  At dim 256 the accumulators leave room for 128 rows and one workgroup.
+        // 2048, 216 -> 132 us; at 8192 rows 356 us against 333).  At dim 256 the accumulators leave room for 128 rows and one workgroup.
         p.many_waves = d.kv.dim == 256 || most_rows <= 128 ? 4 : 8;
         const int64_t bm = 32 * p.many_waves, slots = d.kv.dim < 256 && p.many_waves == 4 ? 512 : 256;
         p.many_tiles = rows / bm + B;

