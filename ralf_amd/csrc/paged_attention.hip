@@ -845,7 +845,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     }
     __syncthreads();            // (s_odd)
 
-    {
+    if (nt) {
         if (s_odd) {            // the values taken out, to the rows that see them
             for (int key = sb * KB; key < se * KB && key < t.L; ++key) {
                 const int pg = table[key >> a.page_log2];
@@ -859,13 +859,22 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
                 if (!(k0 < wg_lo || k0 + KB - 1 > wg_hi || b)) continue;        // (a tile that all see kept them)
                 const int64_t at = pg * head_rows + (int64_t)hk * c.page + (key & (c.page - 1));
                 const uint8_t* vrow = (const uint8_t*)c.v + at * (D * ESZ);
-                const bool nan = STORE >= RALF_KV_E4M3 && ((const uint8_t*)c.v_exp)[at] == 255u;
+                float scale = 1.f;
+                if constexpr (STORE >= RALF_KV_E4M3) scale = exp_value(((const uint8_t*)c.v_exp)[at]);
                 const bool see = key >= lo && key <= hi;
 #pragma unroll
                 for (int ct = 0; ct < D / 32; ++ct)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = nan ? __builtin_nanf("") : STORE == RALF_KV_INT8 ? 0.f : odd_value<STORE>(vrow, 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3));
+                        const int col = 32 * ct + 8 * (i >> 2) + 4 * h + (i & 3);
+                        float x;
+                        if constexpr (STORE == RALF_KV_BF16) x = odd_value<STORE>(vrow, col);
+                        else {          // (an exponent of 255, a NaN code, a product behind fp32's range)
+                            float f[4];
+                            codes_f32<STORE>(vrow[col], f);
+                            x = f[0] * scale;
+                            x = fabsf(x) < __builtin_inff() ? 0.f : x;
+                        }
                         if (see) acc[ct][i] += x;
                         asm volatile("" ::: "memory");      // (one load at a time)
                     }
@@ -942,9 +951,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     else ((bf16*)a.d.o)[at] = (bf16)x;
 }
 
-// How a call is laid out.  A sequence of more than FEW rows under a key head goes to many_kernel: few_kernel reads the keys again for every 16 rows, a tile of
+// How a call is laid out.  A sequence of more than `few` rows under a key head goes to many_kernel: few_kernel reads the keys again for every 16 rows, a tile of
 // many_kernel costs the same whether it holds 32 rows or 256.
-constexpr int FEW = 64;
 struct Plan {
     int splits, few_rows, few_tiles, many_waves;
     int64_t few_grid, many_tiles;       // tiles of 16 and of 32 * many_waves rows; 0: the kernel is not launched
@@ -956,8 +964,12 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     int64_t keys = (int64_t)d.kv.max_pages * d.kv.page;
     if (d.max_kv > 0 && d.max_kv < keys) keys = d.max_kv;
     if (d.causal && d.window > 0 && d.window + 256 < keys) keys = d.window + 256;      // (what a tile can see of them)
+    // 64 rows; 32 where the keys are few and a tile's prologue is most of either kernel (64 sequences on 300 keys, us with 32 against 64: 41 / 62 at up to 96 rows, 42 / 53
+    // at up to 128, but 48 / 42 at up to 48; on 2048 keys 64 is the better one, 115 against 156 at up to 48 rows, on e4m3 87 against 147), and for a single sequence,
+    // which takes one of the kernels alone (48 rows on 32768 keys: 40 against 61, on e4m3 40 against 44)
+    const int few = keys <= 512 || B == 1 ? 32 : 64;
     int64_t s;
-    if (d.dtype == RALF_F32 || most_rows <= FEW) {
+    if (d.dtype == RALF_F32 || most_rows <= few) {
         p.few_rows = 0x7fffffff;
         p.few_grid = rows / 16 + B;
         const int64_t tiles = d.T * ((G + 15) / 16), wgs = (p.few_grid < tiles ? p.few_grid : tiles) * heads;
@@ -975,12 +987,12 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
         const int64_t bm = 32 * p.many_waves, slots = d.kv.dim < 256 && p.many_waves == 4 ? 512 : 256;
         p.many_tiles = rows / bm + B;
         if (B > 1) {
-            p.few_rows = FEW;
-            p.few_tiles = FEW / 16;
-            p.few_grid = B * (FEW / 16);
+            p.few_rows = few;
+            p.few_tiles = few / 16;
+            p.few_grid = B * (few / 16);
         }
         // cut the keys only as far as leaves every CU its workgroups, in pieces of 4 tiles at least
-        const int64_t bound = B * ((most_rows + bm - 1) / bm), other = rows / bm + (B < rows / FEW ? B : rows / FEW);
+        const int64_t bound = B * ((most_rows + bm - 1) / bm), other = rows / bm + (B < rows / few ? B : rows / few);
         const int64_t wgs = (bound < other ? bound : other) * heads;
         s = slots / (wgs > 0 ? wgs : 1);
         if (s > keys / 256) s = keys / 256;
