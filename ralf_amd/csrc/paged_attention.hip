@@ -7,7 +7,10 @@
 // are the operand of the second as they stand (the matrix instruction's contraction slots are named after the keys the lane holds), row maxima need
 // two exchanges (lanes 16 and 32 apart), and every rescaling is lane-local.
 //   bf16: v_mfma_f32_16x16x32_bf16, keys and values rounded to bf16 already (8-bit codes are exact in it, their powers of two go to the scores and the
-//         probabilities in fp32), probabilities rounded to bf16 (half a step: 2^-8; the sum is taken in fp32 before that rounding).
+//         probabilities in fp32).  few_kernel takes a probability as two bf16 parts (2^-16 of it left out), so that a result is off by its own rounding alone: 5 % of
+//         the time at most where 8-bit codes are unpacked, nothing where bytes bound it.  many_kernel rounds it to one (half a step: 2^-8; the sum is taken in fp32
+//         before that rounding): two parts are half as many matrix instructions again and took 429 us against 320 (2048 new on 8192 cached tokens, 32 / 8 heads of 128),
+//         for results that are off by 0.0017 (their own rounding to bf16) instead of 0.0023 of their size.
 //   fp32: v_mfma_f32_16x16x4_f32 on an fp32 cache; on 8-bit codes three bf16 products, the query and the probabilities in three bf16 parts (split3).
 // Running maximum and sum of the softmax in fp32; exponentials base 2 with log2(e) folded into the scale.
 //
@@ -82,7 +85,7 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int w, int lane, int pe
 // few rows: 16 to a workgroup, its 4 waves take blocks of 32 or 64 keys in turn (a long axis and few rows: the keys are what there is to divide).
 // K and V go from memory straight into registers, each byte once per 16 rows; a block's loads are issued a block ahead of its products and its pages looked up
 // two ahead, which keeps 60 - 130 KB in flight to a CU.  Bound by bytes: 64 sequences of 2048 - 8192 tokens, 8 key heads of 128: e4m3 684 MB in 153 us (4.5 TB/s; without
-// the loads ahead 450 us), bf16 4.8 TB/s; a copy reaches 4.9 on this card.
+// the loads ahead 450 us), bf16 4.8 TB/s (282 us); a copy reaches 4.9 on this card.
 // ------------------------------------------------------------------------------------------------
 // The shapes of a lane's share of a block of NT sixteens of keys.  Of a key row it holds EPL consecutive elements (16 bytes) of every 4 EPL -- the contraction over
 // dims may run in any order, as long as the query's registers follow the same one -- and of four value rows of each sixteen CPL columns.
@@ -97,6 +100,7 @@ struct Few {
     // keys of a block: enough bytes in flight with two blocks' registers (loaded one ahead) in 256, the scores' exchanges paid for many keys
     static constexpr bool FP32 = STORE == RALF_KV_F32;              // fp32 products; otherwise bf16 ones, of fp32 queries in three parts
     static constexpr int PARTS = F32 && !FP32 ? 3 : 1;
+    static constexpr int WPARTS = F32 && !FP32 ? 3 : 2;             // of the weights: split2 leaves 2^-16 of one, so that a bf16 result is off by its own rounding alone
     static constexpr int NT = FP32 ? (D * ESZ >= 512 ? 1 : 2) : (D * ESZ >= 128 ? 2 : 4);
     static constexpr int REGS = NT * (NK * KW + 4 * VW);
     static constexpr bool TWO = REGS <= 80;                         // two blocks' registers
@@ -166,6 +170,16 @@ __device__ __forceinline__ void split3(const float* f, bf16x8 (&part)[3]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_perm(w[x][2 * i + 1], w[x][2 * i], 0x07060302u);
         part[x] = __builtin_bit_cast(bf16x8, v);
+    }
+}
+
+// Eight weights as sums of two bf16 values, each rounded to nearest: what is left out is 2^-8 of 2^-8 of a weight
+__device__ __forceinline__ void split2(const float* f, bf16x8 (&part)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bf16 hi = (bf16)f[i];
+        part[0][i] = hi;
+        part[1][i] = (bf16)(f[i] - (float)hi);
     }
 }
 
@@ -380,11 +394,9 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
         } else {
 #pragma unroll
             for (int g = 0; g < NT / 2; ++g) {
-                bf16x8 pb[S::PARTS];
-                if constexpr (S::PARTS == 3) split3(&p[8 * g], pb);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) pb[0][i] = (bf16)p[8 * g + i];
+                bf16x8 pb[S::WPARTS];
+                if constexpr (S::WPARTS == 3) split3(&p[8 * g], pb);
+                else split2(&p[8 * g], pb);
 #pragma unroll
                 for (int q = 0; q < CPL; q += 2) {
                     // columns q, q + 1 of the lane, keys in the order of pb: pairs of keys side by side
@@ -402,7 +414,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
                         }
                     }
 #pragma unroll
-                    for (int y = S::PARTS - 1; y >= 0; --y) {
+                    for (int y = S::WPARTS - 1; y >= 0; --y) {
                         acc[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v0), pb[y], acc[q], 0, 0, 0);
                         acc[q + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v1), pb[y], acc[q + 1], 0, 0, 0);
                     }
