@@ -23,6 +23,9 @@ namespace {
 using namespace paged;
 
 constexpr int MAX_SPLITS = 128;
+// The reference of the exponentials (log2 units) stays so far above the row's largest score that weights are at most 1, 2^-8 as a rule: 256 keys of equal weight may hold fp32's
+// largest number before an unnormalised sum leaves its range.  (More of it would take as much from the other end: sums of values below 2^-118 already leave the normal range.)
+constexpr float HEADROOM = 8.f;
 
 struct Args {
     RalfPagedAttnDesc d;
@@ -349,7 +352,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
         float mx = p[0];
 #pragma unroll
         for (int i = 1; i < 4 * NT; ++i) mx = fmaxf(mx, p[i]);
-        mx = fmaxf(m, wave::max_x16_x32(mx));
+        mx = fmaxf(m, wave::max_x16_x32(mx) + HEADROOM);
         const float base = mx == -__builtin_inff() ? 0.f : mx;
         if (__any(mx > m)) {
             const float alpha = exp2f_(m - base);          // (m = -inf: 0)
@@ -634,8 +637,8 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[i][j] = 0.f;
-    // the reference of the exponentials, in log2 units and always a whole number, so that moving it scales what has been summed up exactly; it follows the largest
-    // score in steps of 8 and more (a weight is then 2^8 at most, which costs fp32 sums and bf16 weights nothing)
+    // the reference of the exponentials, in log2 units and always a whole number, so that moving it scales what has been summed up exactly; set HEADROOM above the largest
+    // score it stays until a score passes it (a weight is then 1 at most)
     float m2 = -__builtin_inff(), l = 0.f;
 
     const int* table = c.table + (int64_t)t.b * c.table_ld;
@@ -732,9 +735,9 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
         float mo = mx;
         wave::swap32(mx, mo);
         mx = __builtin_elementwise_maximum(mx, mo) * qs;
-        const bool need = mx > m2 + 8.f;
+        const bool need = mx > m2;
         if (__any(need)) {
-            const float mn = need ? ceilf(mx) : m2;
+            const float mn = need ? ceilf(mx) + HEADROOM : m2;
             const float alpha = mn == -__builtin_inff() ? 1.f : exp2f_(m2 - mn);       // (m2 = -inf: 0; unchanged: 1)
             m2 = mn;
             l *= alpha;
