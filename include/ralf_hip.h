@@ -581,7 +581,8 @@ int ralf_rope_axes(const RalfRopeDesc* d, void* stream);
 /* key / value cache in pages: k, v [n_pages][heads][page][dim] (contiguous, 16-byte aligned), page in {16, 32, 64, 128, 256}, dim in {32, 64, 128, 256}.
  * store: RALF_KV_F32 / RALF_KV_BF16 hold the values; RALF_KV_E4M3 / RALF_KV_INT8 hold codes, and k_exp, v_exp uint8 [n_pages][heads][page] the power of two
  * 2^(byte - 127) that a row's codes are multiples of.  Rule of a row: e = the smallest integer with max|x| <= 448 * 2^e (127 * 2^e for int8), at least
- * -100; code = x / 2^e rounded to nearest even.  A row that holds an infinity or a NaN is stored as byte 255 and zero codes and reads back as NaN.
+ * -100; code = x / 2^e rounded to nearest even, but to no value past fp32's largest (at e = 120 codes end at 240, for int8 at e = 122 at 63), so that what is held is
+ * finite; codes and bytes of other origin have to keep to that, too.  A row that holds an infinity or a NaN is stored as byte 255 and zero codes and reads back as NaN.
  * table int32 [B][table_ld >= max_pages]: the pages of each sequence; kv_len int32 [B]: its tokens (at most max_pages * page are looked at).
  * A page id outside [0, n_pages) is never followed: nothing is written there, reads give zeros, attention leaves its keys out. */
 #define RALF_KV_F32 0

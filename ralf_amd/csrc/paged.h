@@ -55,6 +55,11 @@ __device__ __forceinline__ uint32_t exp_byte(uint32_t u) {
     const int e = (int)(u >> 23) - (STORE == RALF_KV_E4M3 ? 8 : 6) + ((u & 0x7fffffu) > (STORE == RALF_KV_E4M3 ? 0x600000u : 0x7e0000u) ? 1 : 0);
     return u >= 0x7f800000u ? 255u : (uint32_t)(e < 27 ? 27 : e);
 }
+// the largest code of such a row whose value fp32 holds: at the exponents of fp32's largest numbers the next code, 256 (64), would be 2^128
+template <int STORE>
+__device__ __forceinline__ float largest_code(uint32_t byte) {
+    return STORE == RALF_KV_E4M3 ? (byte == 247u ? 240.f : 448.f) : (byte == 249u ? 63.f : 127.f);
+}
 __device__ __forceinline__ float exp_value(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }            // 2^(byte - 127); 255 gives inf (0 * inf = NaN)
 __device__ __forceinline__ float exp_inverse(uint32_t byte) { return __builtin_bit_cast(float, (254u - byte) << 23); }  // 2^(127 - byte), byte in [1, 253]
 

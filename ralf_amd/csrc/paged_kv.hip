@@ -70,16 +70,18 @@ __device__ __forceinline__ void store_row(const RalfPagedKV& c, bool isv, int64_
         const uint32_t ex = exp_byte<STORE>(m);
         u32x2 code = {0u, 0u};
         if (ex != 255u) {
-            const float inv = exp_inverse(ex);
+            const float inv = exp_inverse(ex), top = largest_code<STORE>(ex);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = __builtin_amdgcn_fmed3f(f[i] * inv, -top, top);       // (nothing is cut off but what would be rounded past fp32's range)
             if constexpr (STORE == RALF_KV_E4M3) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * inv, f[4 * i + 1] * inv, 0, false);
-                    code[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * inv, f[4 * i + 3] * inv, w, true);
+                    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+                    code[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], w, true);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) code[i >> 2] |= ((uint32_t)(int)rintf(f[i] * inv) & 0xffu) << (8 * (i & 3));
+                for (int i = 0; i < 8; ++i) code[i >> 2] |= ((uint32_t)(int)rintf(f[i]) & 0xffu) << (8 * (i & 3));
             }
         }
         *(u32x2*)((uint8_t*)(isv ? c.v : c.k) + row * D + e0) = code;

@@ -66,3 +66,56 @@ def test_attention_mean_of_large_values(store, dtype, n):
     out = ops.paged_attention(rnd(n, 2, 64, seed=1, dtype=dtype).cuda(), pool, table.cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), kv_len.cuda())
     # equal weights, their sum and the value's sum off by a step of fp32 a key at most; the division by two
     assert ((out.double() / 2.0 ** 127 - 1).abs() <= (2 * 200 + 2) * O.U32 + O.half_step(dtype)).all()
+
+
+# ---------------------------------------------------------------------------------------------- the 8-bit stores: no value past fp32's
+LARGEST_FINITE = {E4M3: (240.0, 120), I8: (63.0, 122)}      # the largest code at the exponent that fp32's largest numbers take: 256 and 64 would be 2^128
+
+
+@pytest.mark.parametrize("store", [E4M3, I8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_cache_holds_no_value_past_fp32(store, dtype):
+    from ralf_amd import ops
+
+    top = torch.finfo(dtype).max
+    x = rnd(4, 2, 64, seed=1)
+    x[0, 0, 3], x[0, 1, 0], x[1, 0, 5], x[1, 1, 7] = top, -top, 3.3e38, -3.37e38
+    x[2, 0], x[3, 1, 0] = top, 1.2e38
+    x = x.to(dtype)
+    pool, table, q_start, kv_len = make([4], [4], 2, 64, 16, store, dtype, seed=2)
+    ops.paged_kv_write(pool, x.cuda(), -x.cuda(), table.cuda(), q_start.cuda(), kv_len.cuda())
+    code, e = LARGEST_FINITE[store]
+    for sign, got, exp in ((1, pool.k, pool.k_exp), (-1, pool.v, pool.v_exp)):
+        for t in range(4):
+            c, byte = O.quantise(sign * x[t], store)
+            c = torch.where((byte == 127 + e)[:, None], c.clamp(-code, code), c)       # (the nearest that fp32 holds)
+            assert torch.equal(exp[int(table[0, 0]), :, t].cpu(), byte)
+            assert torch.equal(got[int(table[0, 0]), :, t].float().cpu().double(), c)
+    k, v = ops.paged_kv_read(pool, table.cuda(), kv_len.cuda(), q_start.cuda(), 4, dtype=F32)
+    assert torch.isfinite(k).all() and torch.equal(v, -k)
+    assert k[0, 0, 3].item() == code * 2.0 ** e
+
+
+@pytest.mark.parametrize("store", [E4M3, I8])
+@pytest.mark.parametrize("n,past", [(1, 40), (90, 40), (90, 400)])
+@pytest.mark.parametrize("kw", [{}, dict(causal=False), dict(window=3)])
+def test_attention_agrees_on_the_largest_held_values(store, n, past, kw):
+    """one value of bf16's largest among small ones, seen by some rows or by all, on few and on many rows: the same finite value for both"""
+    from ralf_amd import ops
+
+    L = past + n
+    pool, table, q_start, kv_len = make([L], [L], 1, 64, 16, store, BF16, seed=3)
+    k, v, q = rnd(L, 1, 64, seed=1, dtype=BF16), rnd(L, 1, 64, seed=2, dtype=BF16), rnd(n, 2, 64, seed=4, dtype=BF16)
+    for t in (10, L - 20):
+        v[t, 0, 7] = torch.finfo(BF16).max
+    ops.paged_kv_write(pool, k.cuda(), v.cuda(), table.cuda(), q_start.cuda(), kv_len.cuda())
+    start = torch.tensor([0, n], dtype=torch.int32)
+    many = ops.paged_attention(q.cuda(), pool, table.cuda(), start.cuda(), kv_len.cuda(), **kw)
+    want, e, _ = O.attention(q, *O.pool_values(pool), table, start, kv_len, 0.125, p_step=O.half_step(BF16), **kw)
+    assert torch.isfinite(want).all()
+    O.check(many, want, e + O.half_step(BF16) * (want.abs() + e), "rows together")
+    if kw.get("causal", True):
+        for i in (0, n // 2, n - 1):                       # the same rows alone
+            at = torch.tensor([L - n + i + 1], dtype=torch.int32)
+            one = ops.paged_attention(q[i:i + 1].cuda(), pool, table.cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), at.cuda(), **kw)
+            O.check(one, want[i:i + 1], (e + O.half_step(BF16) * (want.abs() + e))[i:i + 1], "a row alone")
