@@ -57,11 +57,13 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
     }
     const int P = d.R >> 1, j0 = c * N, n = P - j0 < N ? P - j0 : N;
     float cs[N], sn[N];
+    uint32_t stay = 0u;                                 // bit q: the pair's axis has no positions, its elements are copied (1 * a - 0 * b would carry b's infinities and NaN to a)
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         if (q >= n) { cs[q] = 1.f; sn[q] = 0.f; continue; }
         const int ax = d.axis[j0 + q];
         const bool ok = (unsigned)ax < (unsigned)d.A;
+        stay |= (ok ? 0u : 1u) << q;
         const double turns = ok ? (double)d.pos[(int64_t)ax * d.pos_as + t] * (d.freq[j0 + q] * 0.15915494309189533577) : 0.0;
         const float f = (float)(turns - rint(turns));
         float s, co;
@@ -89,6 +91,13 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
                     r[q] = (T)f;
                 }
             }
+            if (stay) {
+#pragma unroll
+                for (int q = 0; q < N; ++q) {           // element q of the two pieces: of pairs q / 2 and (q + N) / 2 where pairs are adjacent
+                    p[q] = (stay >> (ADJ ? q / 2 : q)) & 1u ? u[q] : p[q];
+                    r[q] = (stay >> (ADJ ? (q + N) / 2 : q)) & 1u ? w[q] : r[q];
+                }
+            }
             *(V*)(y + h * d.y_hs + o1) = p;
             *(V*)(y + h * d.y_hs + o2) = r;
         }
@@ -101,9 +110,11 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a) {
                 if (q >= n) continue;
                 const int i1 = ADJ ? 2 * (j0 + q) : j0 + q, i2 = ADJ ? i1 + 1 : P + j0 + q;
                 float e, f;
-                turn((float)xh[i1], (float)xh[i2], cs[q], sn[q], e, f);
-                yh[i1] = (T)e;
-                yh[i2] = (T)f;
+                const T u = xh[i1], w = xh[i2];
+                const bool keep = (stay >> q) & 1u;
+                turn((float)u, (float)w, cs[q], sn[q], e, f);
+                yh[i1] = keep ? u : (T)e;
+                yh[i2] = keep ? w : (T)f;
             }
         }
     }

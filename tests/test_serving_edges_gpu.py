@@ -119,3 +119,35 @@ def test_attention_agrees_on_the_largest_held_values(store, n, past, kw):
             at = torch.tensor([L - n + i + 1], dtype=torch.int32)
             one = ops.paged_attention(q[i:i + 1].cuda(), pool, table.cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda(), at.cuda(), **kw)
             O.check(one, want[i:i + 1], (e + O.half_step(BF16) * (want.abs() + e))[i:i + 1], "a row alone")
+
+
+# ---------------------------------------------------------------------------------------------- rotary positions
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("adjacent", [False, True])
+@pytest.mark.parametrize("P,D", [(8, 20), (16, 32), (11, 22)])
+def test_pairs_of_foreign_axes_stay_as_they_are(dtype, adjacent, P, D):
+    """a pair whose axis has no positions keeps its bits, infinities, NaN and negative zeros included, forwards and backwards, out of and in place"""
+    from ralf_amd import functional, ops
+
+    freq, axis = torch.full((P,), 0.7, dtype=torch.float64), torch.arange(P, dtype=torch.int32) % 2
+    away = [0, 1, P // 2, P - 1]
+    axis[away] = torch.tensor([-1, 2, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
+    x, pos = rnd(5, 3, D, seed=1), torch.randint(1, 99, (2, 5), generator=gen(2))
+    first, second = ([2 * j for j in away], [2 * j + 1 for j in away]) if adjacent else (away, [j + P for j in away])
+    odd = torch.tensor([math.inf, -math.inf, math.nan, -0.0, 3.0, -5.0])
+    for n, (a, b) in enumerate(zip(first, second)):
+        x[..., a], x[..., b] = odd[torch.arange(15) % 6].view(5, 3), odd[(torch.arange(15) // 6 + n + 1) % 6].view(5, 3)
+    x = x.to(dtype).cuda()
+    args = (pos.cuda(), freq.cuda(), axis.cuda())
+    for inverse in (False, True):
+        y = ops.rope_axes(x, *args, adjacent=adjacent, inverse=inverse)
+        assert torch.equal(bits(y[..., first + second]), bits(x[..., first + second]))
+        rest = [i for i in range(D) if i not in first + second]
+        want, e = O.rope(x.cpu(), pos, freq, axis, adjacent, -1 if inverse else 1)
+        O.check(y[..., rest], want[..., rest], (e + O.half_step(dtype) * (want.abs() + e))[..., rest], "the others")
+        z = x.clone()
+        ops.rope_axes(z, *args, adjacent=adjacent, inverse=inverse, out=z)
+        assert torch.equal(bits(z), bits(y))
+    leaf = torch.zeros_like(x, requires_grad=True)
+    g, = torch.autograd.grad(functional.rope_axes(leaf, *args, adjacent), leaf, x)
+    assert torch.equal(bits(g[..., first + second]), bits(x[..., first + second]))
