@@ -626,12 +626,15 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
         const uint32_t flip = a.qscale < 0.f ? 0x80008000u : 0u;      // (a negative scale goes into the query, so that the largest score has the largest weight)
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) {
-            q[j] = live && a.qscale != 0.f ? *(const u32x4*)(qp + 16 * j) : u32x4{0u, 0u, 0u, 0u};
+            q[j] = live ? *(const u32x4*)(qp + 16 * j) : u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[j][i] ^= flip;
+            for (int i = 0; i < 4; ++i) {
+                if (a.qscale == 0.f) q[j][i] = ((q[j][i] & 0x7f80u) == 0x7f80u ? 0x7fc0u : 0u) | ((q[j][i] & 0x7f800000u) == 0x7f800000u ? 0x7fc00000u : 0u);
+                q[j][i] ^= flip;
+            }
         }
     }
-    const float qs = a.qscale == 0.f ? 1.f : fabsf(a.qscale);          // (a scale of 0 is a query of 0: hidden scores are -inf, and stay so)
+    const float qs = a.qscale == 0.f ? 1.f : fabsf(a.qscale);          // (a scale of 0 is a query of 0, and of NaN where it was not finite: hidden scores are -inf, and stay so)
     f32x16 acc[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)

@@ -151,3 +151,20 @@ def test_pairs_of_foreign_axes_stay_as_they_are(dtype, adjacent, P, D):
     leaf = torch.zeros_like(x, requires_grad=True)
     g, = torch.autograd.grad(functional.rope_axes(leaf, *args, adjacent), leaf, x)
     assert torch.equal(bits(g[..., first + second]), bits(x[..., first + second]))
+
+
+# ---------------------------------------------------------------------------------------------- attention: a scale of zero
+@pytest.mark.parametrize("store,dtype", [(F32, F32), (BF16, BF16), (I8, BF16)])
+@pytest.mark.parametrize("n", [1, 100])
+def test_scale_of_zero_keeps_what_is_not_finite(store, dtype, n):
+    """0 * inf is NaN, whichever number of rows; finite rows are the mean of what they see"""
+    from ralf_amd import ops
+
+    pool, table, q_start, kv_len = make([n + 30], [n], 1, 64, 16, store, dtype, seed=3)
+    q, k, v = rnd(n, 2, 64, seed=4, dtype=dtype), rnd(n, 1, 64, seed=5, dtype=dtype), rnd(n, 1, 64, seed=6, dtype=dtype)
+    q[n // 2, 0, 3], q[n // 2, 1, 5] = math.nan, math.inf
+    ops.paged_kv_write(pool, k.cuda(), v.cuda(), table.cuda(), q_start.cuda(), kv_len.cuda())
+    out = ops.paged_attention(q.cuda(), pool, table.cuda(), q_start.cuda(), kv_len.cuda(), scale=0.0)
+    want, e, _ = O.attention(q, *O.pool_values(pool), table, q_start, kv_len, 0.0, p_step=O.half_step(dtype) if dtype == BF16 else 0.0)
+    assert want[n // 2].isnan().all()
+    O.check(out, want, e.nan_to_num() + O.half_step(dtype) * (want.abs() + e).nan_to_num(), "scale 0")
