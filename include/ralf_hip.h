@@ -568,8 +568,8 @@ int ralf_tlayer_pack(const RalfPackJob* jobs, int njobs, void* stream);
  * ------------------------------------------------------------------------------------------- */
 /* rotary positions with several axes: pair j of the first R dims of every head turns by pos[axis[j]][t] * freq[j] radians
  *   (a, b) -> (a cos - b sin, b cos + a sin);  dims >= R pass through.
- * x, y [T][H][D] of `dtype` (RALF_F32 / RALF_BF16) with token / head strides in elements (the last dim contiguous); y may be x itself, otherwise the
- * two must not overlap.  pos int64 [A][pos_as >= T], |pos| < 2^31; freq double [R/2]; axis int32 [R/2] (a pair whose axis is outside [0, A) is not turned).
+ * x, y [T][H][D] of `dtype` (RALF_F32 / RALF_BF16) with token / head strides in elements (the last dim contiguous; y's rows may not overlap one another); y may be
+ * x itself, otherwise the two must not overlap.  pos int64 [A][pos_as >= T], |pos| < 2^31; freq double [R/2]; axis int32 [R/2] (a pair whose axis is outside [0, A) is not turned).
  * adjacent: pair j = dims (2j, 2j+1), otherwise (j, R/2 + j).  inverse: the opposite angle (the gradient of the forward). */
 typedef struct RalfRopeDesc {
     const void* x; void* y; const int64_t* pos; const double* freq; const int* axis;
@@ -604,7 +604,7 @@ int ralf_paged_kv_write(const RalfPagedKV* kv, int dtype, const void* k, const v
 int ralf_paged_kv_read(const RalfPagedKV* kv, int dtype, void* k, void* v, const int* start, int64_t rows, void* stream);
 
 /* attention of each sequence's newest tokens over its pages.  q, o [T][q_heads][dim] of `dtype` (RALF_BF16 with pools of bf16 / e4m3 / int8; RALF_F32 with
- * fp32 / e4m3 / int8), strides in elements, multiples of 8; q_heads a multiple of kv->heads: query head h reads key head h / (q_heads / heads).
+ * fp32 / e4m3 / int8), strides in elements, multiples of 8 (o's rows may not overlap one another); q_heads a multiple of kv->heads: query head h reads key head h / (q_heads / heads).
  * Row i of the n = q_start[b+1] - q_start[b] rows of sequence b stands at position P = kv_len[b] - n + i and sees the keys p with
  *   0 <= p < kv_len[b];  p <= P if causal;  p > P - window if window > 0.
  * o = sum_p exp(s_p - max s) v_p / sum_p exp(s_p - max s), s = scale * q.k; a row that sees no key (or only scores of -inf) gives zeros.  What a row does

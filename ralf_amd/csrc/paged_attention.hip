@@ -18,6 +18,7 @@
 // token's or an out-of-window value that is an infinity or a NaN must not reach a row through 0 * inf: such values are taken out of the products of partly visible
 // blocks and added, behind the loop, to the rows that see them.
 #include "paged.h"
+#include "rows.h"
 
 namespace {
 using namespace paged;
@@ -1087,6 +1088,7 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
     RALF_REQUIRE(d.q_ts % 8 == 0 && d.q_hs % 8 == 0 && d.o_ts % 8 == 0 && d.o_hs % 8 == 0 && (uintptr_t)d.q % 16 == 0 && (uintptr_t)d.o % 16 == 0 &&
                      d.q_ts >= 0 && d.q_hs >= 0 && d.o_ts >= 0 && d.o_hs >= 0,
                  "paged_attention: rows have to start at multiples of 8 elements, 16-byte aligned");
+    RALF_REQUIRE(ralf::rows_apart(d.T, d.o_ts, d.q_heads, d.o_hs, d.kv.dim), "paged_attention: the output's rows overlap");
     Args a;
     a.d = d;
     a.G = d.q_heads / d.kv.heads;

@@ -8,6 +8,7 @@
 //   * bound by bytes: every element is read once and written once in 16-byte pieces: 16384 tokens of 40 heads of 128 in bf16, 336 MB in 74 us (4.5 TB/s); heads of 134 dims
 //     (rows at any element) 3.4 TB/s against 1.8 with single elements.
 #include "common.h"
+#include "rows.h"
 
 namespace {
 typedef __bf16 bf16;
@@ -148,7 +149,7 @@ extern "C" int ralf_rope_axes(const RalfRopeDesc* dp, void* stream) {
     RALF_REQUIRE(d.x_ts >= 0 && d.x_hs >= 0 && d.y_ts >= 0 && d.y_hs >= 0 && d.pos_as >= 0, "rope_axes: negative stride");
     if (d.T == 0) return RALF_OK;
     RALF_REQUIRE(d.x && d.y && d.pos && d.freq && d.axis, "rope_axes: null pointer");
-    RALF_REQUIRE((d.T == 1 || d.y_ts > 0) && (d.H == 1 || d.y_hs > 0), "rope_axes: the output's rows overlap");
+    RALF_REQUIRE(ralf::rows_apart(d.T, d.y_ts, d.H, d.y_hs, d.D), "rope_axes: the output's rows overlap");
     RALF_REQUIRE(d.x != d.y || (d.x_ts == d.y_ts && d.x_hs == d.y_hs), "rope_axes: in place needs one set of strides");
     return d.dtype == RALF_BF16 ? launch<bf16>(d, stream) : launch<float>(d, stream);
 }

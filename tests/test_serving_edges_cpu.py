@@ -1,0 +1,47 @@
+"""Serving operators without a GPU: calls that the C entries refuse before anything is launched, and what they plan."""
+import ctypes
+
+import pytest
+
+from ralf_amd import _lib
+from ralf_amd._abi import RalfPagedAttnDesc, RalfPagedKV, RalfRopeDesc
+
+FAKE = 1 << 20      # an aligned address that nothing may follow
+
+
+def refused(rc, says):
+    assert rc < 0
+    assert says in _lib.lib().ralf_last_error().decode()
+
+
+def paged(**kw):
+    d = RalfPagedKV(k=FAKE, v=FAKE, k_exp=FAKE, v_exp=FAKE, table=FAKE, kv_len=FAKE, n_pages=4, table_ld=2, page=16, heads=2, dim=32, store=1, B=2, max_pages=2)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+def attention(**kw):
+    d = RalfPagedAttnDesc(kv=paged(), q=FAKE, o=2 * FAKE, q_start=FAKE, T=3, q_ts=128, q_hs=32, o_ts=128, o_hs=32, q_heads=4, dtype=1, causal=1, scale=1.0)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+def rope(**kw):
+    d = RalfRopeDesc(x=FAKE, y=2 * FAKE, pos=FAKE, freq=FAKE, axis=FAKE, T=4, x_ts=64, x_hs=32, y_ts=64, y_hs=32, pos_as=4, H=2, D=32, R=32, A=2)
+    for n, v in kw.items():
+        setattr(d, n, v)
+    return d
+
+
+# (strides of [T, heads, 32]: expanded over tokens, over heads; rows that begin within others)
+OVERLAPPING = [(0, 32), (128, 0), (0, 0), (64, 32), (128, 24), (120, 32), (32, 64), (8, 8)]
+
+
+@pytest.mark.parametrize("ts,hs", OVERLAPPING)
+def test_outputs_whose_rows_overlap(ts, hs):
+    """two rows of the output in one place: refused (a workgroup each would write it)"""
+    L = _lib.lib()
+    refused(L.ralf_paged_attention(ctypes.byref(attention(o_ts=ts, o_hs=hs)), None, 0, None), "overlap")
+    refused(L.ralf_rope_axes(ctypes.byref(rope(H=4, x_ts=128, y_ts=ts, y_hs=hs)), None), "overlap")

@@ -168,3 +168,40 @@ def test_scale_of_zero_keeps_what_is_not_finite(store, dtype, n):
     want, e, _ = O.attention(q, *O.pool_values(pool), table, q_start, kv_len, 0.0, p_step=O.half_step(dtype) if dtype == BF16 else 0.0)
     assert want[n // 2].isnan().all()
     O.check(out, want, e.nan_to_num() + O.half_step(dtype) * (want.abs() + e).nan_to_num(), "scale 0")
+
+
+# ---------------------------------------------------------------------------------------------- outputs given by strides
+def test_outputs_whose_rows_overlap_are_refused():
+    from ralf_amd import _lib, ops
+
+    pool, table, q_start, kv_len = make([20, 30], [3, 2], 2, 64, 16, BF16, BF16, seed=2)
+    q = rnd(5, 4, 64, seed=3, dtype=BF16).cuda()
+    args = (pool, table.cuda(), q_start.cuda(), kv_len.cuda())
+    freq, axis = ops.rope_table((32,), device="cuda")
+    pos = torch.arange(5).view(1, 5).cuda()
+    flat = torch.full((5 * 4 * 64,), 7.0, dtype=BF16, device="cuda")
+    for out in (flat[:256].view(1, 4, 64).expand(5, 4, 64), flat[:320].view(5, 1, 64).expand(5, 4, 64), flat.as_strided((5, 4, 64), (192, 64, 1))):
+        with pytest.raises(_lib.RalfHipError, match="overlap"):
+            ops.paged_attention(q, *args, out=out)
+        with pytest.raises(_lib.RalfHipError, match="overlap"):
+            ops.rope_axes(q, pos, freq, axis, out=out)
+    assert bool((flat == 7.0).all())
+
+
+def test_outputs_in_other_orders():
+    """heads outermost, every second head or token of a wider tensor: the same bits"""
+    from ralf_amd import ops
+
+    pool, table, q_start, kv_len = make([90, 300, 40], [3, 100, 1], 2, 64, 16, BF16, BF16, seed=2)
+    T = int(q_start[-1])
+    q = rnd(T, 4, 64, seed=3, dtype=BF16).cuda()
+    args = (pool, table.cuda(), q_start.cuda(), kv_len.cuda())
+    freq, axis = ops.rope_table((32,), device="cuda")
+    pos = torch.arange(T).view(1, T).cuda()
+    for run in (lambda x, **kw: ops.paged_attention(x, *args, **kw), lambda x, **kw: ops.rope_axes(x, pos, freq, axis, **kw)):
+        want = run(q)
+        for wide, view in ((torch.full((4, T, 64), 7.0), lambda t: t.transpose(0, 1)), (torch.full((T, 8, 64), 7.0), lambda t: t[:, 1::2]), (torch.full((2 * T, 4, 64), 7.0), lambda t: t[::2])):
+            wide = wide.to(BF16).cuda()
+            run(q, out=view(wide))
+            assert torch.equal(bits(view(wide)), bits(want))
+            assert bool((wide == 7.0).any()) == (wide.numel() > want.numel())
