@@ -604,7 +604,8 @@ int ralf_paged_kv_write(const RalfPagedKV* kv, int dtype, const void* k, const v
 int ralf_paged_kv_read(const RalfPagedKV* kv, int dtype, void* k, void* v, const int* start, int64_t rows, void* stream);
 
 /* attention of each sequence's newest tokens over its pages.  q, o [T][q_heads][dim] of `dtype` (RALF_BF16 with pools of bf16 / e4m3 / int8; RALF_F32 with
- * fp32 / e4m3 / int8), strides in elements, multiples of 8 (o's rows may not overlap one another); q_heads a multiple of kv->heads: query head h reads key head h / (q_heads / heads).
+ * fp32 / e4m3 / int8), strides in elements, multiples of 8 (o's rows may not overlap one another; o may
+ * be q itself, otherwise the two must not overlap); q_heads a multiple of kv->heads: query head h reads key head h / (q_heads / heads).
  * Row i of the n = q_start[b+1] - q_start[b] rows of sequence b stands at position P = kv_len[b] - n + i and sees the keys p with
  *   0 <= p < kv_len[b];  p <= P if causal;  p > P - window if window > 0.
  * o = sum_p exp(s_p - max s) v_p / sum_p exp(s_p - max s), s = scale * q.k; a row that sees no key (or only scores of -inf) gives zeros.  What a row does
@@ -625,7 +626,7 @@ int ralf_paged_attention(const RalfPagedAttnDesc* d, void* workspace, size_t wor
  * c_out = those at index >= prompt_len[b] (NULL: 0):
  *   x = x > 0 ? x / repetition[b] : x * repetition[b]  where c > 0;   x -= frequency[b] * c_out + (c_out > 0 ? presence[b] : 0);   x += bias[v];
  *   x = -inf where bit (v & 31) of mask[mask_row[b]][v >> 5] is 0 (mask_row NULL: row b; a mask_row outside [0, mask_rows): no mask).
- * logits, out [B][V] of `dtype` with row strides (elements); out may be logits itself.  repetition / presence / frequency float [B], bias float [V] or [B][bias_ld]
+ * logits, out [B][V] of `dtype` with row strides (elements); out may be logits itself, otherwise the two must not overlap.  repetition / presence / frequency float [B], bias float [V] or [B][bias_ld]
  * (bias_ld 0: one row for all), each may be NULL.  len int32 [B] (clamped to [0, L]). */
 typedef struct RalfLogitsDesc {
     const void* logits; void* out; const int64_t* tokens; const int* len; const int* prompt_len;

@@ -6,6 +6,7 @@
 // first, which is why the tile is as wide as leaves every CU workgroups.  64 rows of 130 001 fp32 logits with biases by row and 4096 tokens of history: 103 MB in 24 us
 // (4.3 TB/s; 45 us with single-element loads behind the counting).
 #include "common.h"
+#include "rows.h"
 
 namespace {
 typedef __bf16 bf16;
@@ -113,6 +114,7 @@ extern "C" int ralf_logits_process(const RalfLogitsDesc* dp, void* stream) {
     if (d.B == 0) return RALF_OK;
     RALF_REQUIRE(d.logits && d.out && d.ld_in >= d.V && d.ld_out >= d.V, "logits_process: null logits, or rows shorter than V");
     RALF_REQUIRE(d.logits != d.out || d.ld_in == d.ld_out, "logits_process: in place needs one row stride");
+    RALF_REQUIRE(d.logits == d.out || ralf::rows_disjoint({d.logits, d.ld_in, 0}, {d.out, d.ld_out, 0}, d.B, 1, d.V, d.dtype == RALF_BF16 ? 2 : 4), "logits_process: the output overlaps the logits without being them");
     if (d.repetition || d.presence || d.frequency)
         RALF_REQUIRE(d.len && (d.L == 0 || d.tokens) && d.tok_ld >= d.L, "logits_process: penalties need the history and its lengths");
     RALF_REQUIRE(!d.bias || d.bias_ld == 0 || d.bias_ld >= d.V, "logits_process: bias rows shorter than V");

@@ -1089,6 +1089,8 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
                      d.q_ts >= 0 && d.q_hs >= 0 && d.o_ts >= 0 && d.o_hs >= 0,
                  "paged_attention: rows have to start at multiples of 8 elements, 16-byte aligned");
     RALF_REQUIRE(ralf::rows_apart(d.T, d.o_ts, d.q_heads, d.o_hs, d.kv.dim), "paged_attention: the output's rows overlap");
+    RALF_REQUIRE((d.q == d.o && d.q_ts == d.o_ts && d.q_hs == d.o_hs) || ralf::rows_disjoint({d.q, d.q_ts, d.q_hs}, {d.o, d.o_ts, d.o_hs}, d.T, d.q_heads, d.kv.dim, d.dtype == RALF_BF16 ? 2 : 4),
+                 "paged_attention: the output overlaps the queries without being them");
     Args a;
     a.d = d;
     a.G = d.q_heads / d.kv.heads;

@@ -134,6 +134,7 @@ int launch(const RalfRopeDesc& d, void* stream) {
     a.hg = (int)(want < 1 ? 1 : want > d.H ? d.H : want);
     const int64_t blocks = (per * a.hg + 255) / 256;
     RALF_REQUIRE(blocks < ((int64_t)1 << 31) && (int64_t)(a.rot + a.pass) * a.hg < ((int64_t)1 << 31), "rope_axes: too many elements for one launch");
+    RALF_REQUIRE(d.x == d.y || ralf::rows_disjoint({d.x, d.x_ts, d.x_hs}, {d.y, d.y_ts, d.y_hs}, d.T, d.H, d.D, sizeof(T)), "rope_axes: the output overlaps x without being x");
     if (d.adjacent) rope_kernel<T, true><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
     else rope_kernel<T, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
     return ralf::check_launch("rope_axes");

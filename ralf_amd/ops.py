@@ -1168,7 +1168,7 @@ def rope_table(sections, theta=10000.0, ladder="joint", order="blocks", device=N
 def rope_axes(x, pos, freq, axis, *, adjacent=False, inverse=False, out=None):
     """rotary positions with several axes (ralf_rope_axes): x [T, H, D] fp32 / bf16 (any token / head strides), pos int64 [A, T], freq float64 [P], axis int32 [P]
     (rope_table).  The first 2 P dims of every head are turned -- pairs (j, P + j), or (2j, 2j + 1) with adjacent -- by pos[axis[j], t] * freq[j]; the others pass.
-    inverse: the opposite angle.  out: a tensor of x's shape and type, x itself for in place."""
+    inverse: the opposite angle.  out: a tensor of x's shape and type, x itself for in place (no other overlap with x)."""
     dt = _TORCH2CODE.get(x.dtype)
     assert dt is not None, f"rope_axes: dtype {x.dtype}"
     xs = _rows3(x, "rope_axes")
@@ -1281,7 +1281,7 @@ def paged_attention(q, pool, table, q_start, kv_len, *, scale=None, causal=True,
     first: a token sees its own key), q_heads a multiple of the cache's heads; any token / head strides of multiples of 8, 16-byte aligned, here and in out.  causal: position p sees keys <= p; window > 0: only the last `window` of them.
     q bf16 reads caches of bf16 and 8 bits, q fp32 those of fp32 and 8 bits.  A row without a key gives zeros.  max_q / max_kv: the host's upper bounds of the
     new tokens and of kv_len of one sequence; they steer how the work is split (a captured graph keeps its split), not what is computed.
-    Rows behind q_start[B] are not written."""
+    out: a tensor of q's shape and type, q itself for in place (no other overlap with q).  Rows behind q_start[B] are not written."""
     kv, held = _paged("paged_attention", pool, table, kv_len)
     _starts(q_start, kv.B, "paged_attention: q_start")
     dt = _TORCH2CODE.get(q.dtype)

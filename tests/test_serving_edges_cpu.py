@@ -4,7 +4,7 @@ import ctypes
 import pytest
 
 from ralf_amd import _lib
-from ralf_amd._abi import RalfPagedAttnDesc, RalfPagedKV, RalfRopeDesc
+from ralf_amd._abi import RalfLogitsDesc, RalfPagedAttnDesc, RalfPagedKV, RalfRopeDesc
 
 FAKE = 1 << 20      # an aligned address that nothing may follow
 
@@ -45,3 +45,18 @@ def test_outputs_whose_rows_overlap(ts, hs):
     L = _lib.lib()
     refused(L.ralf_paged_attention(ctypes.byref(attention(o_ts=ts, o_hs=hs)), None, 0, None), "overlap")
     refused(L.ralf_rope_axes(ctypes.byref(rope(H=4, x_ts=128, y_ts=ts, y_hs=hs)), None), "overlap")
+
+
+@pytest.mark.parametrize("size,dtype", [(4, 0), (2, 1)])
+def test_outputs_that_overlap_their_inputs(size, dtype):
+    """an output that lies across its input without being it: refused (some workgroup would read what another has written)"""
+    L = _lib.lib()
+    # x [4, 4, 32] with steps 128, 32: shifted by elements, by a head, by a token, back by a token, by half a byte's element; then with other steps
+    for off, ts, hs in ((size, 128, 32), (32 * size, 128, 32), (128 * size, 128, 32), (-128 * size, 128, 32), (511 * size, 128, 32), (1, 256, 64), (0, 256, 32), (64 * size, 32, 128)):
+        refused(L.ralf_rope_axes(ctypes.byref(rope(H=4, x_ts=128, y=FAKE + off, y_ts=ts, y_hs=hs, dtype=dtype)), None), "in place" if off == 0 else "overlap")
+    # queries in a wider projection, the output over its neighbouring heads
+    for off in (-32 * size, 32 * size, 96 * size, 224 * size):
+        refused(L.ralf_paged_attention(ctypes.byref(attention(kv=paged(store=dtype), q_ts=256, o=FAKE + off, o_ts=256, dtype=dtype)), None, 0, None), "overlap")
+    refused(L.ralf_paged_attention(ctypes.byref(attention(kv=paged(store=dtype), q_ts=256, o=FAKE, o_ts=128, dtype=dtype)), None, 0, None), "overlap")
+    for off, ld in ((size, 8), (-8 * size, 8), (15 * size, 8), (4 * size, 16)):
+        refused(L.ralf_logits_process(ctypes.byref(RalfLogitsDesc(logits=FAKE, out=FAKE + off, ld_in=8 if ld == 8 else 16, ld_out=ld, B=2, V=8, dtype=dtype)), None), "overlap")

@@ -205,3 +205,34 @@ def test_outputs_in_other_orders():
             run(q, out=view(wide))
             assert torch.equal(bits(view(wide)), bits(want))
             assert bool((wide == 7.0).any()) == (wide.numel() > want.numel())
+
+
+def test_outputs_beside_and_in_place_of_their_inputs():
+    """an output among the heads that its input leaves free in one buffer, or the input itself: the same bits, and the input or what lies around it unharmed"""
+    from ralf_amd import ops
+
+    pool, table, q_start, kv_len = make([90, 300, 40, 9000], [3, 100, 1, 1], 2, 64, 16, BF16, BF16, seed=2)
+    T = int(q_start[-1])
+    q = rnd(T, 4, 64, seed=3, dtype=BF16).cuda()
+    args = (pool, table.cuda(), q_start.cuda(), kv_len.cuda())
+    freq, axis = ops.rope_table((32,), device="cuda")
+    pos = torch.arange(T).view(1, T).cuda()
+    for run in (lambda x, **kw: ops.paged_attention(x, *args, **kw), lambda x, **kw: ops.rope_axes(x, pos, freq, axis, **kw)):
+        want = run(q)
+        for src, dst in ((slice(0, 4), slice(4, 8)), (slice(5, 9), slice(1, 5)), (slice(0, 8, 2), slice(1, 9, 2))):
+            wide = torch.full((T, 9, 64), 7.0, dtype=BF16, device="cuda")
+            wide[:, src] = q
+            run(wide[:, src], out=wide[:, dst])
+            assert torch.equal(bits(wide[:, dst]), bits(want)) and torch.equal(bits(wide[:, src]), bits(q))
+        wide = torch.full((T, 6, 64), 7.0, dtype=BF16, device="cuda")
+        wide[:, 1:5] = q
+        run(wide[:, 1:5], out=wide[:, 1:5])
+        assert torch.equal(bits(wide[:, 1:5]), bits(want)) and bool((wide[:, ::5] == 7.0).all())
+        outer = torch.cat([q.transpose(0, 1), torch.full((4, T, 64), 7.0, dtype=BF16, device="cuda")])          # heads outermost
+        run(outer[:4].transpose(0, 1), out=outer[4:].transpose(0, 1))
+        assert torch.equal(bits(outer[4:].transpose(0, 1)), bits(want))
+    x = rnd(6, 1000, seed=1).cuda()
+    bias = rnd(1000, seed=2).cuda()
+    both = torch.cat([x, torch.zeros_like(x)], 1)
+    ops.logits_process(both[:, :1000], bias=bias, out=both[:, 1000:])
+    assert torch.equal(both[:, 1000:], x + bias) and torch.equal(both[:, :1000], x)
