@@ -982,7 +982,7 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     const int64_t most_rows = d.max_q > 0 && d.max_q < d.T ? d.max_q * G : rows;       // (a wrong bound costs time only: each kernel alone takes every sequence)
     int64_t keys = (int64_t)d.kv.max_pages * d.kv.page;
     if (d.max_kv > 0 && d.max_kv < keys) keys = d.max_kv;
-    if (d.causal && d.window > 0 && d.window + 256 < keys) keys = d.window + 256;      // (what a tile can see of them)
+    if (d.causal && d.window > 0 && d.window + (int64_t)256 < keys) keys = d.window + (int64_t)256;      // (what a tile can see of them)
     // 64 rows; 32 where the keys are few and a tile's prologue is most of either kernel (64 sequences on 300 keys, us with 32 against 64: 41 / 62 at up to 96 rows, 42 / 53
     // at up to 128, but 48 / 42 at up to 48; on 2048 keys 64 is the better one, 115 against 156 at up to 48 rows, on e4m3 87 against 147), and for a single sequence,
     // which takes one of the kernels alone (48 rows on 32768 keys: 40 against 61, on e4m3 40 against 44)

@@ -60,3 +60,13 @@ def test_outputs_that_overlap_their_inputs(size, dtype):
     refused(L.ralf_paged_attention(ctypes.byref(attention(kv=paged(store=dtype), q_ts=256, o=FAKE, o_ts=128, dtype=dtype)), None, 0, None), "overlap")
     for off, ld in ((size, 8), (-8 * size, 8), (15 * size, 8), (4 * size, 16)):
         refused(L.ralf_logits_process(ctypes.byref(RalfLogitsDesc(logits=FAKE, out=FAKE + off, ld_in=8 if ld == 8 else 16, ld_out=ld, B=2, V=8, dtype=dtype)), None), "overlap")
+
+
+@pytest.mark.parametrize("dtype,T,max_q", [(0, 3, 0), (1, 3, 0), (1, 3000, 0), (1, 3000, 1)])
+def test_the_widest_windows_plan_like_none(dtype, T, max_q):
+    """windows up to 2^31 - 1, to which larger ones are cut: the split of the keys (seen in the workspace) is the one without a window"""
+    need = lambda w: _lib.lib().ralf_paged_attention_workspace_bytes(ctypes.byref(attention(kv=paged(store=dtype, B=2, max_pages=4096, table_ld=4096, n_pages=4096), dtype=dtype, T=T, max_q=max_q, window=w)))    # noqa: E731
+    assert need(0) > 0
+    for w in (2 ** 31 - 1, 2 ** 31 - 256, 2 ** 31 - 257, 65536):
+        assert need(w) == need(0)
+    assert need(1) < need(0)
