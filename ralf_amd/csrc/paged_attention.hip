@@ -24,6 +24,7 @@ namespace {
 using namespace paged;
 
 constexpr int MAX_SPLITS = 128;
+constexpr float LOG2E = 1.4426950408889634f;
 // The reference of the exponentials (log2 units) stays so far above the row's largest score that weights are at most 1, 2^-8 as a rule: 256 keys of equal weight may hold fp32's
 // largest number before an unnormalised sum leaves its range.  (More of it would take as much from the other end: sums of values below 2^-118 already leave the normal range.)
 constexpr float HEADROOM = 8.f;
@@ -1067,6 +1068,7 @@ int check(const RalfPagedAttnDesc& d) {
     RALF_REQUIRE(d.kv.store >= RALF_KV_E4M3 || d.kv.store == (d.dtype == RALF_F32 ? RALF_KV_F32 : RALF_KV_BF16), "paged_attention: a cache of store %d takes queries of its own type", d.kv.store);
     RALF_REQUIRE(d.q_heads > 0 && d.q_heads % d.kv.heads == 0, "paged_attention: %d query heads on %d key heads", d.q_heads, d.kv.heads);
     RALF_REQUIRE(d.T >= 0 && d.T * d.q_heads < ((int64_t)1 << 31), "paged_attention: %lld rows", (long long)d.T);
+    RALF_REQUIRE(fabsf(d.scale * LOG2E) < __builtin_inff(), "paged_attention: a scale of %g", d.scale);
     RALF_REQUIRE(d.window >= 0 && d.max_q >= 0 && d.max_kv >= 0, "paged_attention: negative window or bound");
     return RALF_OK;
 }
@@ -1100,7 +1102,7 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
     a.few_tiles = p.few_tiles;
     a.page_log2 = __builtin_ctz(d.kv.page);
     if (d.kv.n_pages == 0) a.d.kv.max_pages = 0;        // (no page to look at: every row is empty)
-    a.qscale = d.scale * 1.4426950408889634f;
+    a.qscale = d.scale * LOG2E;
     const size_t need = ralf_paged_attention_workspace_bytes(dp);
     if (need && (!workspace || workspace_bytes < need)) {
         ralf::set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);

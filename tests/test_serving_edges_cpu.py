@@ -70,3 +70,12 @@ def test_the_widest_windows_plan_like_none(dtype, T, max_q):
     for w in (2 ** 31 - 1, 2 ** 31 - 256, 2 ** 31 - 257, 65536):
         assert need(w) == need(0)
     assert need(1) < need(0)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3.4e38])
+def test_scales_that_are_not_finite(scale):
+    """refused, as is one that is not finite once log2(e) is in it (empty rows would be NaN on many rows and zeros on few)"""
+    L = _lib.lib()
+    for kw in (dict(scale=scale), dict(scale=-scale), dict(scale=scale, T=0)):
+        refused(L.ralf_paged_attention(ctypes.byref(attention(**kw)), None, 0, None), "scale")
+    assert L.ralf_paged_attention_workspace_bytes(ctypes.byref(attention(kv=paged(max_pages=4096, table_ld=4096, n_pages=4096), scale=scale))) == 0
