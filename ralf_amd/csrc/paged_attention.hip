@@ -1067,7 +1067,7 @@ int check(const RalfPagedAttnDesc& d) {
     RALF_REQUIRE(d.dtype == RALF_F32 || d.dtype == RALF_BF16, "paged_attention: dtype %d", d.dtype);
     RALF_REQUIRE(d.kv.store >= RALF_KV_E4M3 || d.kv.store == (d.dtype == RALF_F32 ? RALF_KV_F32 : RALF_KV_BF16), "paged_attention: a cache of store %d takes queries of its own type", d.kv.store);
     RALF_REQUIRE(d.q_heads > 0 && d.q_heads % d.kv.heads == 0, "paged_attention: %d query heads on %d key heads", d.q_heads, d.kv.heads);
-    RALF_REQUIRE(d.T >= 0 && d.T * d.q_heads < ((int64_t)1 << 31), "paged_attention: %lld rows", (long long)d.T);
+    RALF_REQUIRE(d.T >= 0 && d.T < ((int64_t)1 << 31) && d.T * d.q_heads < ((int64_t)1 << 31), "paged_attention: %lld rows", (long long)d.T);
     RALF_REQUIRE(fabsf(d.scale * LOG2E) < __builtin_inff(), "paged_attention: a scale of %g", d.scale);
     RALF_REQUIRE(d.window >= 0 && d.max_q >= 0 && d.max_kv >= 0, "paged_attention: negative window or bound");
     return RALF_OK;

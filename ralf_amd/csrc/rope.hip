@@ -129,10 +129,10 @@ int launch(const RalfRopeDesc& d, void* stream) {
     a.rot = (d.R / 2 + n - 1) / n;
     a.pass = d.x == d.y ? 0 : (d.D - d.R + n - 1) / n;
     // one head group = the angles once per token; more of them only as far as the launch would otherwise leave the card's 256 CUs short of threads
-    const int64_t per = (int64_t)(a.rot + a.pass) * d.T;
-    const int64_t want = ((int64_t)1 << 18) / per;
+    const ralf::wide per = (ralf::wide)(a.rot + a.pass) * d.T;
+    const int64_t want = (int64_t)(((int64_t)1 << 18) / per);
     a.hg = (int)(want < 1 ? 1 : want > d.H ? d.H : want);
-    const int64_t blocks = (per * a.hg + 255) / 256;
+    const ralf::wide blocks = (per * a.hg + 255) / 256;
     RALF_REQUIRE(blocks < ((int64_t)1 << 31) && (int64_t)(a.rot + a.pass) * a.hg < ((int64_t)1 << 31), "rope_axes: too many elements for one launch");
     RALF_REQUIRE(d.x == d.y || ralf::rows_disjoint({d.x, d.x_ts, d.x_hs}, {d.y, d.y_ts, d.y_hs}, d.T, d.H, d.D, sizeof(T)), "rope_axes: the output overlaps x without being x");
     if (d.adjacent) rope_kernel<T, true><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(a);
@@ -145,7 +145,7 @@ extern "C" int ralf_rope_axes(const RalfRopeDesc* dp, void* stream) {
     RALF_REQUIRE(dp, "rope_axes: null descriptor");
     const RalfRopeDesc& d = *dp;
     RALF_REQUIRE(d.dtype == RALF_F32 || d.dtype == RALF_BF16, "rope_axes: dtype %d", d.dtype);
-    RALF_REQUIRE(d.T >= 0 && d.H > 0 && d.D > 0 && d.A > 0, "rope_axes: bad sizes");
+    RALF_REQUIRE(d.T >= 0 && d.H > 0 && d.D > 0 && d.D < (1 << 30) && d.A > 0, "rope_axes: bad sizes");
     RALF_REQUIRE(d.R > 0 && d.R % 2 == 0 && d.R <= d.D, "rope_axes: %d rotated dims of %d (an even number of at most the head's is needed)", d.R, d.D);
     RALF_REQUIRE(d.x_ts >= 0 && d.x_hs >= 0 && d.y_ts >= 0 && d.y_hs >= 0 && d.pos_as >= 0, "rope_axes: negative stride");
     if (d.T == 0) return RALF_OK;

@@ -79,3 +79,13 @@ def test_scales_that_are_not_finite(scale):
     for kw in (dict(scale=scale), dict(scale=-scale), dict(scale=scale, T=0)):
         refused(L.ralf_paged_attention(ctypes.byref(attention(**kw)), None, 0, None), "scale")
     assert L.ralf_paged_attention_workspace_bytes(ctypes.byref(attention(kv=paged(max_pages=4096, table_ld=4096, n_pages=4096), scale=scale))) == 0
+
+
+@pytest.mark.parametrize("T", [1 << 61, 1 << 62, (1 << 62) + 1, (1 << 63) - 1])
+def test_row_counts_whose_products_wrap(T):
+    """counts that pass 2^63 once multiplied are refused like other large ones"""
+    L = _lib.lib()
+    refused(L.ralf_rope_axes(ctypes.byref(rope(T=T)), None), "too many")
+    refused(L.ralf_paged_attention(ctypes.byref(attention(T=T)), None, 0, None), "rows")
+    assert L.ralf_paged_attention_workspace_bytes(ctypes.byref(attention(T=T))) == 0
+    refused(L.ralf_rope_axes(ctypes.byref(rope(D=(1 << 31) - 1, R=2, T=1)), None), "sizes")
