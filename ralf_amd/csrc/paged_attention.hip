@@ -29,14 +29,21 @@ constexpr float LOG2E = 1.4426950408889634f;
 // largest number before an unnormalised sum leaves its range.  (More of it would take as much from the other end: sums of values below 2^-118 already leave the normal range.)
 constexpr float HEADROOM = 8.f;
 
+// What a kernel leaves of rows whose keys it cuts into several pieces (splits > 1): o [splits][rows][dim] unnormalised, ml [splits][rows][2] reference (log2 units) and sum
+struct Part {
+    float* o;
+    float* ml;
+    int64_t rows;       // T * q_heads; of few_kernel beside many_kernel: B * few_rows * heads, row r of sequence b under key head hk at (b * few_rows + r) * heads + hk
+    int splits;
+    __host__ __device__ size_t bytes(int dim) const { return splits > 1 ? (size_t)splits * rows * (dim + 2) * sizeof(float) : 0; }
+};
 struct Args {
     RalfPagedAttnDesc d;
-    int G, splits, page_log2;
+    int G, page_log2;
     int few_rows;       // sequences of at most so many rows go to few_kernel, the others to many_kernel
     int few_tiles;      // tiles of a sequence in few_kernel's grid where few_rows bounds them; 0: found from q_start
     float qscale;       // scale * log2(e)
-    float* part_o;      // [splits][T * q_heads][dim] unnormalised
-    float* part_ml;     // [splits][T * q_heads][2] running maximum (log2 units), sum
+    Part few, many;
 };
 
 __device__ __forceinline__ float exp2f_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -204,9 +211,9 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, kg = lane >> 4;
     const RalfPagedKV& c = a.d.kv;
-    const int split = blockIdx.x % a.splits;
-    const int hk = (blockIdx.x / a.splits) % c.heads;
-    const Tile t = find_tile<BM>(a, blockIdx.x / a.splits / c.heads, lane, a.few_tiles);
+    const int split = blockIdx.x % a.few.splits;
+    const int hk = (blockIdx.x / a.few.splits) % c.heads;
+    const Tile t = find_tile<BM>(a, blockIdx.x / a.few.splits / c.heads, lane, a.few_tiles);
     if (!t.ok || t.rows > a.few_rows) return;
     const int64_t tok0 = t.tok0;
     const int row = t.row0 + r16;
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
     const int full_lo = behind(p1, a.d.window), full_hi = a.d.causal && p0 < t.L - 1 ? p0 : t.L - 1;   // keys that every row of the tile sees
     // this split's blocks of KB keys
     const int blk0 = kbeg / KB, nblk = kend > kbeg ? (kend + KB - 1) / KB - blk0 : 0;
-    const int per = (nblk + a.splits - 1) / a.splits;
+    const int per = (nblk + a.few.splits - 1) / a.few.splits;
     const int sb = blk0 + split * per, se = sb + per < blk0 + nblk ? sb + per : blk0 + nblk;
 
     const int64_t qoff = (tok0 + ti) * a.d.q_ts + hq * a.d.q_hs;
@@ -508,11 +515,11 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
 #pragma unroll
         for (int q = 0; q < CPL; ++q) o[q] += fw[w] * sm[(w * 16 + orow) * D + oc + 16 * q];
     const int oti = (t.row0 + orow) / a.G, ohq = hk * a.G + (t.row0 + orow) % a.G;
-    if (a.splits > 1) {
-        const int64_t at = ((int64_t)split * a.d.T + tok0 + oti) * a.d.q_heads + ohq;
+    if (a.few.splits > 1) {
+        const int64_t slot = a.few_tiles ? ((int64_t)t.b * a.few_rows + t.row0 + orow) * c.heads + hk : (tok0 + oti) * a.d.q_heads + ohq, at = split * a.few.rows + slot;
 #pragma unroll
-        for (int q = 0; q < CPL; ++q) a.part_o[at * D + oc + 16 * q] = o[q];
-        if (oc == 0) { a.part_ml[at * 2] = mm; a.part_ml[at * 2 + 1] = ll; }
+        for (int q = 0; q < CPL; ++q) a.few.o[at * D + oc + 16 * q] = o[q];
+        if (oc == 0) { a.few.ml[at * 2] = mm; a.few.ml[at * 2 + 1] = ll; }
     } else {
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         const int64_t at = (tok0 + oti) * a.d.o_ts + ohq * a.d.o_hs;
@@ -597,7 +604,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     // tiles of one key head and split side by side on one XCD (workgroups are dealt to the 8 XCDs in turn): they read the same keys
     const int nwg = gridDim.x, q8 = nwg >> 3, r8 = nwg & 7, xcd = blockIdx.x & 7;
     const int vid = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
-    const int hk = vid / ntiles / a.splits, split = vid / ntiles % a.splits;
+    const int hk = vid / ntiles / a.many.splits, split = vid / ntiles % a.many.splits;
     const Tile t = find_tile<M::BM>(a, vid % ntiles, lane, 0);
     if (!t.ok || t.rows <= a.few_rows) return;
     if (threadIdx.x == 0) s_odd = 0;        // (a barrier ahead of the first value stored)
@@ -619,7 +626,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     const Range own = w0 < t.rows ? range(w0, 32) : Range{0, 0, 0, -1};
     const int kbeg = all.kbeg, kend = all.kend, wg_lo = all.lo, wg_hi = all.hi, full_lo = own.lo, full_hi = own.hi;
     const int blk0 = kbeg / KB, nblk = kend > kbeg ? (kend + KB - 1) / KB - blk0 : 0;
-    const int per = (nblk + a.splits - 1) / a.splits;
+    const int per = (nblk + a.many.splits - 1) / a.many.splits;
     const int sb = blk0 + split * per, se = sb + per < blk0 + nblk ? sb + per : blk0 + nblk;
 
     u32x4 q[D / 16];
@@ -906,14 +913,14 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     float lo2 = l;
     wave::swap32(l, lo2);
     l += lo2;
-    if (a.splits > 1) {
-        const int64_t at = ((int64_t)split * a.d.T + tok0 + ti) * a.d.q_heads + hq;
+    if (a.many.splits > 1) {
+        const int64_t at = split * a.many.rows + (tok0 + ti) * a.d.q_heads + hq;
 #pragma unroll
         for (int ct = 0; ct < D / 32; ++ct)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                *(f32x4*)(a.part_o + at * D + 32 * ct + 8 * g + 4 * h) = f32x4{acc[ct][4 * g], acc[ct][4 * g + 1], acc[ct][4 * g + 2], acc[ct][4 * g + 3]};
-        if (h == 0) { a.part_ml[at * 2] = m2; a.part_ml[at * 2 + 1] = l; }
+                *(f32x4*)(a.many.o + at * D + 32 * ct + 8 * g + 4 * h) = f32x4{acc[ct][4 * g], acc[ct][4 * g + 1], acc[ct][4 * g + 2], acc[ct][4 * g + 3]};
+        if (h == 0) { a.many.ml[at * 2] = m2; a.many.ml[at * 2 + 1] = l; }
     } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         bf16* op = (bf16*)a.d.o + (tok0 + ti) * a.d.o_ts + hq * a.d.o_hs;
@@ -929,21 +936,37 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void many_kernel(const 
     }
 }
 
-// The splits of a row joined, a workgroup to a row: the splits' maxima and sums give each its weight (LDS), then their sums are added up, several splits at once
+// The splits of one kernel's rows joined, a workgroup to a row of its Part: the splits' maxima and sums give each its weight (LDS), then their sums are added up, several splits at once
 // and eight loads of each in flight.
-template <int D, bool F32>
-__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+enum JoinRows { ALL, FEW_BESIDE_MANY, MANY_BESIDE_FEW };      // whose rows: of the one kernel that runs, or of one of the two
+template <int D, bool F32, JoinRows ROWS>
+__global__ __launch_bounds__(256) void join_kernel(const Args a, const Part p) {
     constexpr int LANES = D / 4;                                    // threads of a split's row, 4 columns each
     constexpr int WAYS = 256 / LANES;                               // splits at once
     __shared__ float so[WAYS][D], weight[MAX_SPLITS], red[4][2];
-    const int64_t R = a.d.T * a.d.q_heads, r = blockIdx.x;
-    const int64_t t = r / a.d.q_heads;
-    const int h = (int)(r - t * a.d.q_heads);
-    if (t < a.d.q_start[0] || t >= a.d.q_start[a.d.kv.B]) return;
+    const int64_t r = blockIdx.x, R = p.rows;
+    int64_t t;
+    int h;
+    if constexpr (ROWS == FEW_BESIDE_MANY) {
+        const int hk = (int)(r % a.d.kv.heads), row = (int)(r / a.d.kv.heads % a.few_rows), b = (int)(r / a.d.kv.heads / a.few_rows);
+        const int64_t s = a.d.q_start[b], e0 = a.d.q_start[b + 1], e = e0 < a.d.T ? e0 : a.d.T, rows = (e - s) * a.G;
+        if (s < 0 || row >= rows || rows > a.few_rows) return;
+        t = s + row / a.G;
+        h = hk * a.G + row % a.G;
+    } else {
+        t = r / a.d.q_heads;
+        h = (int)(r - t * a.d.q_heads);
+        if (t < a.d.q_start[0] || t >= a.d.q_start[a.d.kv.B]) return;
+        if constexpr (ROWS == MANY_BESIDE_FEW) {        // (not few_kernel's)
+            const Owner w = owner_of(a.d.q_start + 1, a.d.kv.kv_len, a.d.kv.B, t, threadIdx.x & 63);
+            const int64_t e = w.end < a.d.T ? w.end : a.d.T;
+            if (w.b >= a.d.kv.B || (e - a.d.q_start[w.b]) * a.G <= a.few_rows) return;
+        }
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     static_assert(MAX_SPLITS <= 256, "one thread to a split's maximum");
-    const bool have = tid < a.splits;
-    const float ms = have ? a.part_ml[((int64_t)tid * R + r) * 2] : -__builtin_inff(), ls = have ? a.part_ml[((int64_t)tid * R + r) * 2 + 1] : 0.f;
+    const bool have = tid < p.splits;
+    const float ms = have ? p.ml[((int64_t)tid * R + r) * 2] : -__builtin_inff(), ls = have ? p.ml[((int64_t)tid * R + r) * 2 + 1] : 0.f;
     const float wm = wave::max64(ms);
     if (lane == 0) red[wave][0] = wm;
     __syncthreads();
@@ -956,9 +979,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
     const float ll = (red[0][1] + red[1][1]) + (red[2][1] + red[3][1]);
     const int way = tid / LANES, ln = tid % LANES;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    const float* src = a.part_o + r * D + 4 * ln;
+    const float* src = p.o + r * D + 4 * ln;
 #pragma unroll 8
-    for (int s = way; s < a.splits; s += WAYS) o += *(const f32x4*)(src + (int64_t)s * R * D) * weight[s];
+    for (int s = way; s < p.splits; s += WAYS) o += *(const f32x4*)(src + (int64_t)s * R * D) * weight[s];
     *(f32x4*)&so[way][4 * ln] = o;
     __syncthreads();
     if (tid >= D) return;
@@ -974,7 +997,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
 // How a call is laid out.  A sequence of more than `few` rows under a key head goes to many_kernel: few_kernel reads the keys again for every 16 rows, a tile of
 // many_kernel costs the same whether it holds 32 rows or 256.
 struct Plan {
-    int splits, few_rows, few_tiles, many_waves;
+    int few_splits, many_splits, few_rows, few_tiles, many_waves;
     int64_t few_grid, many_tiles;       // tiles of 16 and of 32 * many_waves rows; 0: the kernel is not launched
 };
 inline Plan plan_for(const RalfPagedAttnDesc& d) {
@@ -988,66 +1011,82 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     // at up to 128, but 48 / 42 at up to 48; on 2048 keys 64 is the better one, 115 against 156 at up to 48 rows, on e4m3 87 against 147), and for a single sequence,
     // which takes one of the kernels alone (48 rows on 32768 keys: 40 against 61, on e4m3 40 against 44)
     const int few = keys <= 512 || B == 1 ? 32 : 64;
-    int64_t s;
+    // Splits of few_kernel's keys between wgs workgroups.  A wave takes `turns` blocks of 32 keys one behind the other; two workgroups to a CU run at once.  Splitting costs the
+    // join (5 us, some 6 turns), so short axes stay whole; longer ones are cut until the card is full or a wave has two turns left, and to 16 turns at most, so that
+    // sequences of different lengths even out (64 sequences of 2048 - 8192: 154 us against 162 in one piece) -- but no further than 4096 workgroups, which even out by
+    // themselves.
+    auto few_splits = [&](int64_t wgs) {
+        const int64_t turns = (keys + 127) / 128;
+        const int64_t fill = (512 + wgs - 1) / wgs, enough = (4096 + wgs - 1) / wgs, even = (turns + 15) / 16 < enough ? (turns + 15) / 16 : enough;
+        const int64_t s = fill < turns / 2 ? fill : turns / 2;
+        return turns < 8 ? 1 : s > even ? s : even;
+    };
+    auto bounded = [](int64_t s) { return (int)(s > MAX_SPLITS ? MAX_SPLITS : s < 1 ? 1 : s); };
+    p.few_splits = p.many_splits = 1;
     if (d.dtype == RALF_F32 || most_rows <= few) {
         p.few_rows = 0x7fffffff;
         p.few_grid = rows / 16 + B;
-        const int64_t tiles = d.T * ((G + 15) / 16), wgs = (p.few_grid < tiles ? p.few_grid : tiles) * heads;
-        // Splits of the keys.  A wave takes `turns` blocks of 32 keys one behind the other; two workgroups to a CU run at once.  Splitting costs the join (5 us, some 6
-        // turns), so short axes stay whole; longer ones are cut until the card is full or a wave has two turns left, and to 16 turns at most, so that sequences of
-        // different lengths even out (64 sequences of 2048 - 8192: 154 us against 162 in one piece) -- but no further than 4096 workgroups, which even out by themselves.
-        const int64_t turns = (keys + 127) / 128;
-        const int64_t fill = (512 + wgs - 1) / wgs, enough = (4096 + wgs - 1) / wgs, even = (turns + 15) / 16 < enough ? (turns + 15) / 16 : enough;
-        s = fill < turns / 2 ? fill : turns / 2;
-        s = turns < 8 ? 1 : s > even ? s : even;
+        const int64_t tiles = d.T * ((G + 15) / 16);
+        p.few_splits = bounded(few_splits((p.few_grid < tiles ? p.few_grid : tiles) * heads));
     } else {
         // 256 rows to a workgroup, one of them to a CU; 128 and two to a CU where no sequence has more (half of the waves would only wait: 64 chunks of 32 tokens on
         // 2048, 216 -> 132 us; at 8192 rows 356 us against 333).  At dim 256 the accumulators leave room for 128 rows and one workgroup.
         p.many_waves = d.kv.dim == 256 || most_rows <= 128 ? 4 : 8;
         const int64_t bm = 32 * p.many_waves, slots = d.kv.dim < 256 && p.many_waves == 4 ? 512 : 256;
         p.many_tiles = rows / bm + B;
-        if (B > 1) {
+        // Sequences of few rows beside those of many: single tokens as a rule, one tile to a key head.  Their keys are cut as if they were alone -- few_kernel runs behind
+        // many_kernel and has the card to itself (2048 new tokens on 10 240 and one on 131 072: 417 us, 303 and 103 alone; with many_kernel's one piece 2258) -- and not at all
+        // if the host's bound leaves no such sequence.  Four prompts of up to 512 tokens on 4096, none of them short, pay 5 us of 152 for the workgroups that find nothing to do.
+        if (B > 1 && (d.max_q <= 0 || (d.T - (B - 1) * d.max_q) * G <= few)) {
             p.few_rows = few;
             p.few_tiles = few / 16;
             p.few_grid = B * (few / 16);
+            p.few_splits = bounded(few_splits(B * heads));
         }
         // cut the keys only as far as leaves every CU its workgroups, in pieces of 4 tiles at least
         const int64_t bound = B * ((most_rows + bm - 1) / bm), other = rows / bm + (B < rows / few ? B : rows / few);
         const int64_t wgs = (bound < other ? bound : other) * heads;
-        s = slots / (wgs > 0 ? wgs : 1);
-        if (s > keys / 256) s = keys / 256;
+        const int64_t s = slots / (wgs > 0 ? wgs : 1);
+        p.many_splits = bounded(s > keys / 256 ? keys / 256 : s);
     }
-    s = s > MAX_SPLITS ? MAX_SPLITS : s;
-    p.splits = (int)(s < 1 ? 1 : s);
     return p;
 }
+inline Part part_few(const RalfPagedAttnDesc& d, const Plan& p) {
+    return Part{nullptr, nullptr, p.few_tiles ? (int64_t)d.kv.B * p.few_rows * d.kv.heads : d.T * d.q_heads, p.few_grid ? p.few_splits : 1};
+}
+inline Part part_many(const RalfPagedAttnDesc& d, const Plan& p) { return Part{nullptr, nullptr, d.T * d.q_heads, p.many_splits}; }
 
 template <int D, int STORE, int W>
 int launch_many(const Args& a, const Plan& p, hipStream_t st) {
     constexpr int lds = Many<D, W>::LDS;
     if (lds >= 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(many_kernel<D, STORE, W>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    many_kernel<D, STORE, W><<<(int)(p.many_tiles * a.d.kv.heads * a.splits), 64 * W, lds, st>>>(a, (int)p.many_tiles);
+    many_kernel<D, STORE, W><<<(int)(p.many_tiles * a.d.kv.heads * a.many.splits), 64 * W, lds, st>>>(a, (int)p.many_tiles);
     return ralf::check_launch("paged_attention (many rows)");
 }
 template <int D, int STORE, bool F32>
 int launch(const Args& a, const Plan& p, void* stream) {
     const int64_t heads = a.d.kv.heads;
-    RALF_REQUIRE(p.few_grid * heads * a.splits < ((int64_t)1 << 31) && p.many_tiles * heads * a.splits < ((int64_t)1 << 31), "paged_attention: too many tiles");
+    RALF_REQUIRE(p.few_grid * heads * a.few.splits < ((int64_t)1 << 31) && p.many_tiles * heads * a.many.splits < ((int64_t)1 << 31), "paged_attention: too many tiles");
     hipStream_t st = (hipStream_t)stream;
+    // (a workgroup to a row: T * q_heads < 2^31 of them, and B * heads workgroups of few rows beside many are cut up only below 4096)
+    auto join = [&](const Part& part, auto rows) {
+        join_kernel<D, F32, (JoinRows)rows.value><<<(int)part.rows, 256, 0, st>>>(a, part);
+        return ralf::check_launch("paged_attention (join)");
+    };
     if constexpr (!F32) {
         if (p.many_tiles) {
-            const int rc = D < 256 && p.many_waves == 8 ? launch_many<D, STORE, D < 256 ? 8 : 4>(a, p, st) : launch_many<D, STORE, 4>(a, p, st);
+            int rc = D < 256 && p.many_waves == 8 ? launch_many<D, STORE, D < 256 ? 8 : 4>(a, p, st) : launch_many<D, STORE, 4>(a, p, st);
+            if (!rc && a.many.splits > 1) rc = a.few_tiles ? join(a.many, Const<MANY_BESIDE_FEW>{}) : join(a.many, Const<ALL>{});
             if (rc) return rc;
         }
     }
     if (p.few_grid) {
-        few_kernel<D, STORE, F32><<<(int)(p.few_grid * heads * a.splits), 256, 4 * 16 * D * sizeof(float), st>>>(a);
-        const int rc = ralf::check_launch("paged_attention");
+        few_kernel<D, STORE, F32><<<(int)(p.few_grid * heads * a.few.splits), 256, 4 * 16 * D * sizeof(float), st>>>(a);
+        int rc = ralf::check_launch("paged_attention");
+        if (!rc && a.few.splits > 1) rc = a.few_tiles ? join(a.few, Const<FEW_BESIDE_MANY>{}) : join(a.few, Const<ALL>{});
         if (rc) return rc;
     }
-    if (a.splits == 1) return RALF_OK;
-    join_kernel<D, F32><<<(int)(a.d.T * a.d.q_heads), 256, 0, st>>>(a);
-    return ralf::check_launch("paged_attention (join)");
+    return RALF_OK;
 }
 template <int D>
 int launch_dim(const Args& a, const Plan& p, void* stream) {
@@ -1076,8 +1115,8 @@ int check(const RalfPagedAttnDesc& d) {
 
 extern "C" size_t ralf_paged_attention_workspace_bytes(const RalfPagedAttnDesc* d) {
     if (!d || check(*d) || d->T == 0 || d->kv.B == 0) return 0;
-    const int s = plan_for(*d).splits;
-    return s > 1 ? (size_t)s * d->T * d->q_heads * (d->kv.dim + 2) * sizeof(float) : 0;
+    const Plan p = plan_for(*d);
+    return part_few(*d, p).bytes(d->kv.dim) + part_many(*d, p).bytes(d->kv.dim);
 }
 
 extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace, size_t workspace_bytes, void* stream) {
@@ -1097,7 +1136,8 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
     a.d = d;
     a.G = d.q_heads / d.kv.heads;
     const Plan p = plan_for(d);
-    a.splits = p.splits;
+    a.few = part_few(d, p);
+    a.many = part_many(d, p);
     a.few_rows = p.few_rows;
     a.few_tiles = p.few_tiles;
     a.page_log2 = __builtin_ctz(d.kv.page);
@@ -1108,8 +1148,13 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
         ralf::set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return RALF_ERR_WORKSPACE;
     }
-    a.part_o = (float*)workspace;
-    a.part_ml = need ? (float*)workspace + (size_t)a.splits * d.T * d.q_heads * d.kv.dim : nullptr;
+    float* at = (float*)workspace;
+    for (Part* part : {&a.few, &a.many}) {
+        if (part->splits == 1) continue;
+        part->o = at;
+        part->ml = at + (size_t)part->splits * part->rows * d.kv.dim;
+        at += part->bytes(d.kv.dim) / sizeof(float);
+    }
     switch (d.kv.dim) {
         case 32: return launch_dim<32>(a, p, stream);
         case 64: return launch_dim<64>(a, p, stream);

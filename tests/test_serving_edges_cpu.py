@@ -89,3 +89,19 @@ def test_row_counts_whose_products_wrap(T):
     refused(L.ralf_paged_attention(ctypes.byref(attention(T=T)), None, 0, None), "rows")
     assert L.ralf_paged_attention_workspace_bytes(ctypes.byref(attention(T=T))) == 0
     refused(L.ralf_rope_axes(ctypes.byref(rope(D=(1 << 31) - 1, R=2, T=1)), None), "sizes")
+
+
+def test_single_tokens_beside_a_chunk_keep_their_splits():
+    """one token on 131 072 keys has them cut into as many pieces beside a chunk of 2048 as alone (the workspace holds the pieces of up to 64 rows of every sequence and key head)"""
+    L = _lib.lib()
+
+    def need(T, B, max_q, max_kv=131072):
+        c = paged(B=B, heads=8, dim=128, page=64, max_pages=2048, table_ld=2048, n_pages=4096)
+        return L.ralf_paged_attention_workspace_bytes(ctypes.byref(attention(kv=c, q_heads=32, T=T, max_q=max_q, max_kv=max_kv)))
+
+    alone = need(1, 1, 1) // (1 * 32 * (128 + 2) * 4)
+    assert alone > 8
+    beside = need(2049, 2, 2048)
+    assert beside % (2 * 64 * 8 * (128 + 2) * 4) == 0 and alone // 2 <= beside // (2 * 64 * 8 * (128 + 2) * 4) <= alone
+    assert need(4096, 2, 2048) == 0             # two chunks of 2048: no short sequence
+    assert need(2049, 2, 2048, 512) == 0        # short axes stay whole

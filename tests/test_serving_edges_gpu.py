@@ -236,3 +236,28 @@ def test_outputs_beside_and_in_place_of_their_inputs():
     both = torch.cat([x, torch.zeros_like(x)], 1)
     ops.logits_process(both[:, :1000], bias=bias, out=both[:, 1000:])
     assert torch.equal(both[:, 1000:], x + bias) and torch.equal(both[:, :1000], x)
+
+
+# ---------------------------------------------------------------------------------------------- attention: chunks beside single tokens, both with their keys cut
+@pytest.mark.parametrize("lens,new,Hq,heads,dim,kw", [
+    ([5000, 9000], [100, 1], 2, 1, 64, dict(max_q=100, max_kv=9000)), ([9000, 300, 5000, 0, 40], [1, 200, 16, 0, 3], 4, 2, 64, {}), ([6000, 6000, 6000], [33, 16, 17], 4, 1, 128, dict(max_q=33, max_kv=6000)),
+    ([3000, 4000], [70, 1], 4, 2, 256, dict(window=900)), ([3000, 5000, 2000], [70, 2, 65], 2, 2, 32, dict(causal=False)), ([2500, 2600], [150, 120], 2, 1, 64, dict(max_q=150, max_kv=2600)),
+    ([2500, 2600], [150, 1], 2, 1, 64, dict(max_q=76, max_kv=2600))])
+@pytest.mark.parametrize("store", [BF16, E4M3, I8])
+def test_mixed_batches_with_cut_keys(lens, new, Hq, heads, dim, kw, store):
+    """rows of both kernels, each with splits of its own; two rows behind the last sequence stay; in place of the queries the same bits"""
+    from ralf_amd import ops
+
+    pool, table, q_start, kv_len = make(lens, new, heads, dim, 64, store, BF16, seed=len(lens))
+    T = int(q_start[-1])
+    q, k, v = (rnd(T + 2, h, dim, seed=i, dtype=BF16) for i, h in ((1, Hq), (2, heads), (3, heads)))
+    args = (pool, table.cuda(), q_start.cuda(), kv_len.cuda())
+    ops.paged_kv_write(pool, k.cuda(), v.cuda(), *args[1:])
+    out = torch.full_like(q, 3.0).cuda()
+    ops.paged_attention(q.cuda(), *args, out=out, **kw)
+    assert bool((out[T:] == 3.0).all())
+    want, e, _ = O.attention(q[:T], *O.pool_values(pool), table, q_start, kv_len, dim ** -0.5, p_step=O.half_step(BF16), causal=kw.get("causal", True), window=kw.get("window", 0))
+    O.check(out[:T], want, e + O.half_step(BF16) * (want.abs() + e) + 1e-37, "mixed")
+    same = q.cuda()
+    ops.paged_attention(same, *args, out=same, **kw)
+    assert torch.equal(bits(same[:T]), bits(out[:T])) and torch.equal(bits(same[T:]), bits(q[T:]))
