@@ -261,3 +261,32 @@ def test_mixed_batches_with_cut_keys(lens, new, Hq, heads, dim, kw, store):
     same = q.cuda()
     ops.paged_attention(same, *args, out=same, **kw)
     assert torch.equal(bits(same[:T]), bits(out[:T])) and torch.equal(bits(same[T:]), bits(q[T:]))
+
+
+# ---------------------------------------------------------------------------------------------- a packed projection
+@pytest.mark.parametrize("store", [BF16, E4M3])
+def test_decode_on_a_packed_projection(store):
+    """query and key heads rotated where they lie in the projection, keys and values stored and queries taken as slices of it: the bits of separate tensors"""
+    from ralf_amd import ops
+
+    Hq, Hk, D = 8, 2, 64
+    lens, new = [40, 7, 300], [1, 7, 100]
+    T = sum(new)
+    qkv = rnd(T, Hq + 2 * Hk, D, seed=1, dtype=BF16).cuda()
+    freq, axis = ops.rope_table((8, 24), device="cuda")
+    pos = torch.randint(0, 400, (2, T), generator=gen(2)).cuda()
+    outs = []
+    for packed in (True, False):
+        pool, table, q_start, kv_len = make(lens, new, Hk, D, 16, store, BF16, seed=4)
+        args = (table.cuda(), q_start.cuda(), kv_len.cuda())
+        if packed:
+            x = qkv.clone()
+            ops.rope_axes(x[:, :Hq + Hk], pos, freq, axis, out=x[:, :Hq + Hk])
+            q, k, v = x[:, :Hq], x[:, Hq:Hq + Hk], x[:, Hq + Hk:]
+            assert torch.equal(v, qkv[:, Hq + Hk:])
+        else:
+            q, k, v = (t.contiguous() for t in (qkv[:, :Hq], qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:]))
+            q, k = ops.rope_axes(q, pos, freq, axis), ops.rope_axes(k, pos, freq, axis)
+        ops.paged_kv_write(pool, k, v, *args)
+        outs.append(ops.paged_attention(q, pool, *args, max_q=100, max_kv=300))
+    assert torch.equal(bits(outs[0]), bits(outs[1]))
