@@ -609,7 +609,8 @@ int ralf_paged_kv_read(const RalfPagedKV* kv, int dtype, void* k, void* v, const
  * Row i of the n = q_start[b+1] - q_start[b] rows of sequence b stands at position P = kv_len[b] - n + i and sees the keys p with
  *   0 <= p < kv_len[b];  p <= P if causal;  p > P - window if window > 0.
  * o = sum_p exp(s_p - max s) v_p / sum_p exp(s_p - max s), s = scale * q.k (scale finite); a row that sees no key (or only scores of -inf) gives zeros.  What a row does
- * not see does not reach it, infinities and NaN included.  Finite values give a finite result while sum_p exp(s_p - max s) |v_p| is one that fp32 holds.  Rows at or behind q_start[B] of o are left as they were.
+ * not see does not reach it, infinities and NaN included.  Finite values give a finite result while sum_p exp(s_p - max s) |v_p| is one that fp32 holds;
+ * an infinity that a row does see may reach it as NaN where its weight is too small for fp32.  Rows at or behind q_start[B] of o are left as they were.
  * max_q, max_kv: upper bounds of n and kv_len known to the host (0 = unknown): they steer the split of the work, never the result's definition.
  * workspace: ralf_paged_attention_workspace_bytes() bytes (0 = none needed), 16-byte aligned, private to this call until it has run. */
 typedef struct RalfPagedAttnDesc {

@@ -4,7 +4,8 @@
 // maximum of the bit patterns (ordered like the values, infinities and NaN on top), takes the exponent from its bits, and scales by a power of two -- exact, so
 // only the one rounding to the code remains and every reader gets the same value.  Both kernels are bound by bytes; a wave takes whole tokens, so that finding
 // the sequence (64 probes in one load) and the page is paid once per token and not per row.  42 500 tokens of 2 x 8 x 128 e4m3 -> bf16: 261 MB in 53 us (4.9 TB/s);
-// 10 600 tokens bf16 -> e4m3: 50 MB in 17 us (3 TB/s: a wave's chain of three trips to memory, and rows that lie 128 bytes in each of many pages).
+// 10 600 tokens bf16 -> e4m3: 65 MB in 18 us behind a kernel that has filled the caches with other data, 14 alone (a wave's chain of three trips to memory; it takes one
+// token's rows of all heads, so its stores are 128 bytes in as many places of a page).
 #include "paged.h"
 
 namespace {

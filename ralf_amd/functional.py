@@ -1039,6 +1039,7 @@ def _capturing():
 def rope_axes(x, pos, freq, axis, adjacent=False):
     """ops.rope_axes with a gradient for x.  Refused for a LEAF that requires one while a graph is being captured: if an eager autograd graph of that leaf is still
     alive, its gradient accumulator belongs to the stream of that time, the captured backward would have to wait on it, and the process ends when the capture does.
+    (Every leaf is refused, one without such a graph, too; and the same holds for any leaf further back that x was made from, which is not looked for here.)
     The gradient of a rotation is ops.rope_axes(dy, ..., inverse=True), which can be captured."""
     if x.requires_grad and x.is_leaf and torch.is_grad_enabled() and _capturing():
         raise RuntimeError("rope_axes: the gradient of a leaf inside a graph capture; use ops.rope_axes(dy, ..., inverse=True) there, or pass the leaf without requires_grad")
