@@ -7,8 +7,8 @@
 // are the operand of the second as they stand (the matrix instruction's contraction slots are named after the keys the lane holds), row maxima need
 // two exchanges (lanes 16 and 32 apart), and every rescaling is lane-local.
 //   bf16: v_mfma_f32_16x16x32_bf16, keys and values rounded to bf16 already (8-bit codes are exact in it, their powers of two go to the scores and the
-//         probabilities in fp32).  few_kernel takes a probability as two bf16 parts (2^-16 of it left out), so that a result is off by its own rounding alone: 5 % of
-//         the time at most where 8-bit codes are unpacked, nothing where bytes bound it.  many_kernel rounds it to one (half a step: 2^-8; the sum is taken in fp32
+//         probabilities in fp32).  few_kernel takes a probability as two bf16 parts (2^-16 of it left out), so that a result is off by its own rounding alone: up to
+//         10 % of the time at dims 32 and 64 and where 8-bit codes are unpacked, nothing where bytes bound it.  many_kernel rounds it to one (half a step: 2^-8; the sum is taken in fp32
 //         before that rounding): two parts are half as many matrix instructions again and took 429 us against 320 (2048 new on 8192 cached tokens, 32 / 8 heads of 128),
 //         for results that are off by 0.0017 (their own rounding to bf16) instead of 0.0023 of their size.
 //   fp32: v_mfma_f32_16x16x4_f32 on an fp32 cache; on 8-bit codes three bf16 products, the query and the probabilities in three bf16 parts (split3).
@@ -185,14 +185,32 @@ __device__ __forceinline__ void split3(const float* f, bf16x8 (&part)[3]) {
     }
 }
 
-// Eight weights as sums of two bf16 values, each rounded to nearest: what is left out is 2^-8 of 2^-8 of a weight
+// Eight weights as sums of two bf16 values, each rounded to nearest: what is left out is 2^-8 of 2^-8 of a weight.  The first one's rounding on the bits (ties upwards) holds few_kernel
+// to 128 registers, four waves to a SIMD, on bf16 caches of dims 32 and 64 (134 with the conversion: 64 sequences with 12 new on 2048 keys at dim 32 34 us, 30 so); on 8-bit
+// ones of dim 32 it is the conversion that leaves a wave more (163 registers against 171: 46 us against 50).
+template <bool BITS>
 __device__ __forceinline__ void split2(const float* f, bf16x8 (&part)[2]) {
+    u32x4 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bf16 hi = (bf16)f[i];
-        part[0][i] = hi;
-        part[1][i] = (bf16)(f[i] - (float)hi);
+    for (int i = 0; i < 4; ++i) {
+        const float x = f[2 * i], y = f[2 * i + 1];
+        float xh, yh;
+        if constexpr (BITS) {
+            const uint32_t a = __float_as_uint(x) + 0x8000u, b = __float_as_uint(y) + 0x8000u;
+            xh = __uint_as_float(a & 0xffff0000u);
+            yh = __uint_as_float(b & 0xffff0000u);
+            hi[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        } else {
+            const bf16x2 h = {(bf16)x, (bf16)y};
+            xh = (float)h[0];
+            yh = (float)h[1];
+            hi[i] = __builtin_bit_cast(uint32_t, h);
+        }
+        const bf16x2 rest = {(bf16)(x - xh), (bf16)(y - yh)};
+        lo[i] = __builtin_bit_cast(uint32_t, rest);
     }
+    part[0] = __builtin_bit_cast(bf16x8, hi);
+    part[1] = __builtin_bit_cast(bf16x8, lo);
 }
 
 template <int D, int STORE, bool F32>
@@ -408,7 +426,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
             for (int g = 0; g < NT / 2; ++g) {
                 bf16x8 pb[S::WPARTS];
                 if constexpr (S::WPARTS == 3) split3(&p[8 * g], pb);
-                else split2(&p[8 * g], pb);
+                else split2<STORE == RALF_KV_BF16>(&p[8 * g], pb);
 #pragma unroll
                 for (int q = 0; q < CPL; q += 2) {
                     // columns q, q + 1 of the lane, keys in the order of pb: pairs of keys side by side
