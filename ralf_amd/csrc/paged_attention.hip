@@ -33,8 +33,9 @@ constexpr float HEADROOM = 8.f;
 struct Part {
     float* o;
     float* ml;
-    int64_t rows;       // T * q_heads; of few_kernel beside many_kernel: B * few_rows * heads, row r of sequence b under key head hk at (b * few_rows + r) * heads + hk
+    int64_t rows;       // row t * q_heads + h of all T * q_heads; or `slots`, of few_kernel beside many_kernel where that is fewer:
     int splits;
+    bool slots;         // row (b * few_rows + r) * heads + hk of all B * few_rows * heads, r of sequence b under key head hk
     __host__ __device__ size_t bytes(int dim) const { return splits > 1 ? (size_t)splits * rows * (dim + 2) * sizeof(float) : 0; }
 };
 struct Args {
@@ -534,7 +535,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
         for (int q = 0; q < CPL; ++q) o[q] += fw[w] * sm[(w * 16 + orow) * D + oc + 16 * q];
     const int oti = (t.row0 + orow) / a.G, ohq = hk * a.G + (t.row0 + orow) % a.G;
     if (a.few.splits > 1) {
-        const int64_t slot = a.few_tiles ? ((int64_t)t.b * a.few_rows + t.row0 + orow) * c.heads + hk : (tok0 + oti) * a.d.q_heads + ohq, at = split * a.few.rows + slot;
+        const int64_t own = a.few.slots ? ((int64_t)t.b * a.few_rows + t.row0 + orow) * c.heads + hk : (tok0 + oti) * a.d.q_heads + ohq, at = split * a.few.rows + own;
 #pragma unroll
         for (int q = 0; q < CPL; ++q) a.few.o[at * D + oc + 16 * q] = o[q];
         if (oc == 0) { a.few.ml[at * 2] = mm; a.few.ml[at * 2 + 1] = ll; }
@@ -962,7 +963,7 @@ __global__ __launch_bounds__(256, 8) void join_kernel(const Args a, const Part p
     constexpr int LANES = D / 4;                                    // threads of a split's row, 4 columns each
     constexpr int WAYS = 256 / LANES;                               // splits at once
     __shared__ float so[WAYS][D], weight[MAX_SPLITS], red[4][2];
-    const uint32_t r = blockIdx.x;
+    uint32_t r = blockIdx.x;            // (FEW_BESIDE_MANY: a slot, whichever way the rows lie)
     const int64_t R = p.rows;
     int64_t t;
     int h;
@@ -973,6 +974,7 @@ __global__ __launch_bounds__(256, 8) void join_kernel(const Args a, const Part p
         if (s < 0 || row >= rows || rows > a.few_rows) return;
         t = s + row / a.G;
         h = hk * a.G + row % a.G;
+        if (!p.slots) r = (uint32_t)(t * a.d.q_heads + h);
     } else {
         t = r / (uint32_t)a.d.q_heads;
         h = (int)(r - (uint32_t)t * (uint32_t)a.d.q_heads);
@@ -1072,9 +1074,11 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
     return p;
 }
 inline Part part_few(const RalfPagedAttnDesc& d, const Plan& p) {
-    return Part{nullptr, nullptr, p.few_tiles ? (int64_t)d.kv.B * p.few_rows * d.kv.heads : d.T * d.q_heads, p.few_grid ? p.few_splits : 1};
+    const int64_t all = d.T * d.q_heads, slots = (int64_t)d.kv.B * p.few_rows * d.kv.heads;
+    const bool fewer = p.few_tiles && slots < all;
+    return Part{nullptr, nullptr, fewer ? slots : all, p.few_grid ? p.few_splits : 1, fewer};
 }
-inline Part part_many(const RalfPagedAttnDesc& d, const Plan& p) { return Part{nullptr, nullptr, d.T * d.q_heads, p.many_splits}; }
+inline Part part_many(const RalfPagedAttnDesc& d, const Plan& p) { return Part{nullptr, nullptr, d.T * d.q_heads, p.many_splits, false}; }
 
 template <int D, int STORE, int W>
 int launch_many(const Args& a, const Plan& p, hipStream_t st) {
@@ -1088,9 +1092,10 @@ int launch(const Args& a, const Plan& p, void* stream) {
     const int64_t heads = a.d.kv.heads;
     RALF_REQUIRE(p.few_grid * heads * a.few.splits < ((int64_t)1 << 31) && p.many_tiles * heads * a.many.splits < ((int64_t)1 << 31), "paged_attention: too many tiles");
     hipStream_t st = (hipStream_t)stream;
-    // (a workgroup to a row: T * q_heads < 2^31 of them, and B * heads workgroups of few rows beside many are cut up only below 4096)
+    // (a workgroup to a row: T * q_heads < 2^31 of them; few rows beside many are cut up only where B * heads < 4096)
     auto join = [&](const Part& part, auto rows) {
-        join_kernel<D, F32, (JoinRows)rows.value><<<(int)part.rows, 256, 0, st>>>(a, part);
+        const int64_t wgs = rows.value == FEW_BESIDE_MANY ? a.d.kv.B * (int64_t)a.few_rows * heads : part.rows;
+        join_kernel<D, F32, (JoinRows)rows.value><<<(int)wgs, 256, 0, st>>>(a, part);
         return ralf::check_launch("paged_attention (join)");
     };
     if constexpr (!F32) {
@@ -1168,12 +1173,16 @@ extern "C" int ralf_paged_attention(const RalfPagedAttnDesc* dp, void* workspace
         ralf::set_error("paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return RALF_ERR_WORKSPACE;
     }
-    float* at = (float*)workspace;
-    for (Part* part : {&a.few, &a.many}) {
+    float* at = (float*)workspace;      // the sums (of whole 128-byte rows) of both in front of the references
+    for (Part* part : {&a.many, &a.few}) {
         if (part->splits == 1) continue;
         part->o = at;
-        part->ml = at + (size_t)part->splits * part->rows * d.kv.dim;
-        at += part->bytes(d.kv.dim) / sizeof(float);
+        at += (size_t)part->splits * part->rows * d.kv.dim;
+    }
+    for (Part* part : {&a.many, &a.few}) {
+        if (part->splits == 1) continue;
+        part->ml = at;
+        at += (size_t)part->splits * part->rows * 2;
     }
     switch (d.kv.dim) {
         case 32: return launch_dim<32>(a, p, stream);

@@ -242,10 +242,10 @@ def test_outputs_beside_and_in_place_of_their_inputs():
 @pytest.mark.parametrize("lens,new,Hq,heads,dim,kw", [
     ([5000, 9000], [100, 1], 2, 1, 64, dict(max_q=100, max_kv=9000)), ([9000, 300, 5000, 0, 40], [1, 200, 16, 0, 3], 4, 2, 64, {}), ([6000, 6000, 6000], [33, 16, 17], 4, 1, 128, dict(max_q=33, max_kv=6000)),
     ([3000, 4000], [70, 1], 4, 2, 256, dict(window=900)), ([3000, 5000, 2000], [70, 2, 65], 2, 2, 32, dict(causal=False)), ([2500, 2600], [150, 120], 2, 1, 64, dict(max_q=150, max_kv=2600)),
-    ([2500, 2600], [150, 1], 2, 1, 64, dict(max_q=76, max_kv=2600))])
+    ([2500, 2600], [150, 1], 2, 1, 64, dict(max_q=76, max_kv=2600)), ([3000] * 12, [70] + [1] * 11, 4, 2, 64, dict(max_q=70, max_kv=3000)), ([2000, 3000, 2500], [67, 1, 1], 1, 1, 32, {})])
 @pytest.mark.parametrize("store", [BF16, E4M3, I8])
 def test_mixed_batches_with_cut_keys(lens, new, Hq, heads, dim, kw, store):
-    """rows of both kernels, each with splits of its own; two rows behind the last sequence stay; in place of the queries the same bits"""
+    """rows of both kernels, each with splits of its own (their partial sums by token, or by sequence where that takes less); two rows behind the last sequence stay; in place of the queries the same bits"""
     from ralf_amd import ops
 
     pool, table, q_start, kv_len = make(lens, new, heads, dim, 64, store, BF16, seed=len(lens))
@@ -261,6 +261,39 @@ def test_mixed_batches_with_cut_keys(lens, new, Hq, heads, dim, kw, store):
     same = q.cuda()
     ops.paged_attention(same, *args, out=same, **kw)
     assert torch.equal(bits(same[:T]), bits(out[:T])) and torch.equal(bits(same[T:]), bits(q[T:]))
+
+
+@pytest.mark.parametrize("q_starts", [([0, 100, 101, 101], [0, 3, 60, 101], [0, 0, 1, 101], [0, 33, 66, 99]), ([0, 1, 101, 101], [0, 50, 101, 101], [0, 101, 101, 101])])
+def test_captured_mixed_call_follows_its_starts(q_starts):
+    """a call of both kernels in a graph: replayed with other starts, sequences change sides and every replay has the eager call's bits; eager calls of the same kind in between"""
+    from ralf_amd import ops
+
+    lens, heads, dim = [3000, 5000, 2500], 2, 64
+    pool, table, _, kv_len = make(lens, lens, heads, dim, 64, BF16, BF16, seed=9, garbage=False)
+    k, v = (rnd(sum(lens), heads, dim, seed=i, dtype=BF16).cuda() for i in (1, 2))
+    table, kv_len = table.cuda(), kv_len.cuda()
+    ops.paged_kv_write(pool, k, v, table, torch.tensor([0] + lens).cumsum(0).int().cuda(), kv_len)
+    q, start = rnd(101, 4, dim, seed=3, dtype=BF16).cuda(), torch.tensor(q_starts[0], dtype=torch.int32).cuda()
+    call = lambda: ops.paged_attention(q, pool, table, start, kv_len, max_q=100, max_kv=5000)    # noqa: E731
+    st = ops.own_stream("serving_edges_test")
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        out = call()
+    for turn in range(2):
+        for s in q_starts:
+            start.copy_(torch.tensor(s, dtype=torch.int32))
+            n = s[-1]
+            want = call()[:n].clone()
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out[:n]), bits(want)) and not out[n:].any()
+            ref, e, _ = O.attention(q[:n].cpu(), *O.pool_values(pool), table.cpu(), s, kv_len.cpu(), dim ** -0.5, p_step=O.half_step(BF16))
+            O.check(want, ref, e + O.half_step(BF16) * (ref.abs() + e) + 1e-37, "mixed")
 
 
 # ---------------------------------------------------------------------------------------------- a packed projection
