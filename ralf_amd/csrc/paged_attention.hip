@@ -559,7 +559,7 @@ __global__ __launch_bounds__(256, (Few<D, STORE, F32>::WAVES)) void few_kernel(c
 //   * LDS rows of dim elements without padding, their 16-byte chunks swizzled (kswz, vswz).
 //   * scores run half a tile ahead of their weights and products half a tile behind, step by step in one stream of instructions: the vector unit's 16 exponentials a
 //     lane and half (as long as 8 matrix instructions) run in the matrix unit's shadow.
-// 2048 new on 8192 cached tokens, 32 / 8 heads of 128: 302 - 330 us from box to box, 1020 - 940 TFLOP/s (a large plain product: 1611), both units half busy at a clock of 2.0 GHz.  Left out one at a
+// 2048 new on 8192 cached tokens, 32 / 8 heads of 128: 302 - 330 us from card to card, 1020 - 940 TFLOP/s (a large plain product: 1611), both units half busy at a clock of 2.0 GHz.  Left out one at a
 // time: staging - 46 us, weights - 43, settling - 11; bare matrix instructions, LDS reads and barriers 229 us.  Loads straight into LDS (6 us slower), fragments 4 or 6
 // steps ahead, two workgroups of 4 waves to a CU (+ 23) and other wave priorities gained nothing.
 // ------------------------------------------------------------------------------------------------
