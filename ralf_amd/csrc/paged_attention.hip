@@ -8,7 +8,7 @@
 // two exchanges (lanes 16 and 32 apart), and every rescaling is lane-local.
 //   bf16: v_mfma_f32_16x16x32_bf16, keys and values rounded to bf16 already (8-bit codes are exact in it, their powers of two go to the scores and the
 //         probabilities in fp32).  few_kernel takes a probability as two bf16 parts (2^-16 of it left out), so that a result is off by its own rounding alone: up to
-//         10 % of the time at dims 32 and 64 and where 8-bit codes are unpacked, nothing where bytes bound it.  many_kernel rounds it to one (half a step: 2^-8; the sum is taken in fp32
+//         8 % of the time at dims 32 and 64 and where 8-bit codes are unpacked, nothing where bytes bound it.  many_kernel rounds it to one (half a step: 2^-8; the sum is taken in fp32
 //         before that rounding): two parts are half as many matrix instructions again and took 429 us against 320 (2048 new on 8192 cached tokens, 32 / 8 heads of 128),
 //         for results that are off by 0.0017 (their own rounding to bf16) instead of 0.0023 of their size.
 //   fp32: v_mfma_f32_16x16x4_f32 on an fp32 cache; on 8-bit codes three bf16 products, the query and the probabilities in three bf16 parts (split3).
@@ -186,28 +186,28 @@ __device__ __forceinline__ void split3(const float* f, bf16x8 (&part)[3]) {
     }
 }
 
-// Eight weights as sums of two bf16 values, each rounded to nearest: what is left out is 2^-8 of 2^-8 of a weight.  The first one's rounding on the bits (ties upwards) holds few_kernel
-// to 128 registers, four waves to a SIMD, on bf16 caches of dims 32 and 64 (134 with the conversion: 64 sequences with 12 new on 2048 keys at dim 32 34 us, 30 so); on 8-bit
-// ones of dim 32 it is the conversion that leaves a wave more (163 registers against 171: 46 us against 50).
-template <bool BITS>
+// Eight weights as sums of two bf16 values, 2^-16 of a weight left out.
+//   INF (values that may be infinite: weight times infinity has to be infinity in both parts): the first part by cutting off, so that the rest is not negative, and 2^-22 of the weight
+//     more than the rest, so that it is zero only where the weight is.
+//   otherwise (8-bit codes; their NaN is NaN for any weight): both parts rounded to nearest.
+// On bf16 caches of dims 32 and 64 the first form also holds few_kernel to 128 registers, four waves to a SIMD (134 with the conversion: 64 sequences with 12 new on 2048 keys at
+// dim 32 34 us, 30 so); on 8-bit ones of dim 32 it is the second that leaves a wave more (163 registers against 171: 46 us against 50).
+template <bool INF>
 __device__ __forceinline__ void split2(const float* f, bf16x8 (&part)[2]) {
     u32x4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float x = f[2 * i], y = f[2 * i + 1];
-        float xh, yh;
-        if constexpr (BITS) {
-            const uint32_t a = __float_as_uint(x) + 0x8000u, b = __float_as_uint(y) + 0x8000u;
-            xh = __uint_as_float(a & 0xffff0000u);
-            yh = __uint_as_float(b & 0xffff0000u);
-            hi[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        bf16x2 rest;
+        if constexpr (INF) {
+            constexpr float MORE = 1.f + 0x1p-22f;
+            hi[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+            rest = bf16x2{(bf16)fmaf(x, MORE, -__uint_as_float(__float_as_uint(x) & 0xffff0000u)), (bf16)fmaf(y, MORE, -__uint_as_float(__float_as_uint(y) & 0xffff0000u))};
         } else {
             const bf16x2 h = {(bf16)x, (bf16)y};
-            xh = (float)h[0];
-            yh = (float)h[1];
             hi[i] = __builtin_bit_cast(uint32_t, h);
+            rest = bf16x2{(bf16)(x - (float)h[0]), (bf16)(y - (float)h[1])};
         }
-        const bf16x2 rest = {(bf16)(x - xh), (bf16)(y - yh)};
         lo[i] = __builtin_bit_cast(uint32_t, rest);
     }
     part[0] = __builtin_bit_cast(bf16x8, hi);

@@ -29,6 +29,27 @@ def test_few_rows_round_only_their_result(lens, new, Hq, heads, dim, kw, store):
     O.check(out, want, e + O.half_step(BF16) * (want.abs() + e) + 1e-37, "two parts")
 
 
+@pytest.mark.parametrize("store,dtype", [(F32, F32), (BF16, BF16), (E4M3, BF16), (I8, F32)])
+@pytest.mark.parametrize("n,past", [(1, 300), (3, 300), (100, 600), (1, 5000)])
+@pytest.mark.parametrize("kw", [{}, dict(causal=False)])
+def test_infinities_that_every_row_sees(store, dtype, n, past, kw):
+    """infinite values far behind the newest tokens: infinities of their sign for all rows, NaN where both signs meet (8-bit rows that hold one: NaN), and the other columns as they are"""
+    from ralf_amd import ops
+
+    L = past + n
+    pool, table, q_start, kv_len = make([L], [L], 2, 64, 16, store, dtype, seed=3)
+    k, v, q = rnd(L, 2, 64, seed=1, dtype=dtype), rnd(L, 2, 64, seed=2, dtype=dtype), rnd(n, 4, 64, seed=4, dtype=dtype)
+    for t, c, x in ((5, 1, math.inf), (70, 2, -math.inf), (71, 3, math.inf), (150, 3, -math.inf), (200, 4, math.nan), (201, 63, math.inf)):
+        v[t, 0, c] = x
+    ops.paged_kv_write(pool, k.cuda(), v.cuda(), table.cuda(), q_start.cuda(), kv_len.cuda())
+    start = torch.tensor([0, n], dtype=torch.int32)
+    out = ops.paged_attention(q.cuda(), pool, table.cuda(), start.cuda(), kv_len.cuda(), **kw)
+    want, e, _ = O.attention(q, *O.pool_values(pool), table, start, kv_len, 0.125, p_step=O.half_step(BF16) if dtype == BF16 else 0.0, **kw)
+    if store.itemsize > 1:
+        assert want[:, :2].isinf().sum() == n * 2 * 3 and want[:, :2].isnan().sum() == n * 2 * 2
+    O.check(out, want, (e + O.half_step(dtype) * (want.abs() + e)).nan_to_num(), "infinities")
+
+
 # ---------------------------------------------------------------------------------------------- attention: values near fp32's end
 @pytest.mark.parametrize("store,dtype", [(F32, F32), (BF16, BF16), (E4M3, BF16), (E4M3, F32), (I8, BF16), (I8, F32)])
 @pytest.mark.parametrize("n,past", [(1, 60), (100, 60), (300, 300), (1, 5000), (100, 5000)])
