@@ -1059,7 +1059,7 @@ inline Plan plan_for(const RalfPagedAttnDesc& d) {
         // Sequences of few rows beside those of many: single tokens as a rule, one tile to a key head.  Their keys are cut as if they were alone -- few_kernel runs behind
         // many_kernel and has the card to itself (2048 new tokens on 10 240 and one on 131 072: 417 us, 303 and 103 alone; with many_kernel's one piece 2258) -- and not at all
         // if the host's bound leaves no such sequence.  Four prompts of up to 512 tokens on 4096, none of them short, pay 5 us of 152 for the workgroups that find nothing to do.
-        if (B > 1 && (d.max_q <= 0 || (d.T - (B - 1) * d.max_q) * G <= few)) {
+        if (B > 1 && (d.max_q <= 0 || d.T - (B - 1) * d.max_q <= few / G)) {
             p.few_rows = few;
             p.few_tiles = few / 16;
             p.few_grid = B * (few / 16);

@@ -105,5 +105,6 @@ def test_single_tokens_beside_a_chunk_keep_their_splits():
     assert beside % (2 * 64 * 8 * (128 + 2) * 4) == 0 and alone // 2 <= beside // (2 * 64 * 8 * (128 + 2) * 4) <= alone
     c = lambda T: need(T, 40, 100, 8192)    # noqa: E731
     assert c(139) % (139 * 32 * (128 + 2) * 4) == 0 and 0 < c(139) <= 16 * 139 * 32 * (128 + 2) * 4        # by token where those are fewer
+    assert need(2049, 2, 2 ** 31 - 1) == beside
     assert need(4096, 2, 2048) == 0             # two chunks of 2048: no short sequence
     assert need(2049, 2, 2048, 512) == 0        # short axes stay whole
